@@ -449,6 +449,69 @@ int ukv_snapkv_scores_from_stats(const void* q_obs, const int64_t* q_strides, co
                                  int dtype, const float* obs_stats, float* scores, int64_t scores_stride,
                                  void* workspace, size_t workspace_bytes, ukv_stream_t stream);
 
+/*
+ * The 8-bit cache: K and V of one layer as codes and exponents.
+ *   k, v                codes [num_pages, 16, num_heads, head_dim], one byte each: int8 (UKV_CACHE_INT8) or e4m3,
+ *                       the OCP 8-bit float with a largest value of 448 (UKV_CACHE_FP8)
+ *   k_scale, v_scale    uint8 [num_pages, num_heads, ceil(head_dim / 32), 16]: the exponent byte of 32 dims of
+ *                       each of a page's sixteen tokens, those sixteen contiguous
+ *   layer_strides       twelve byte strides: page, token, head of k and of v, then page, head, block of k_scale
+ *                       and of v_scale
+ * A code c under byte s is the value c * 2^(s - 127), or NaN where s is 255. With A the largest magnitude
+ * of a block of 32 dims and M = 127 or 448, writing takes the smallest e with M * 2^e >= A, within [-24, 9] (int8)
+ * or [-15, 7] (e4m3), stores e + 127, and rounds each x * 2^-e to the nearest code, ties to even; magnitudes
+ * beyond M (above 65024 or 57344, the highest exponents' ends) become M. A block with a NaN or an infinity gets
+ * byte 255. Every value is exact in fp16 and in bf16, so reading does not round, and writing what was read
+ * gives the same values again.
+ */
+#define UKV_CACHE_INT8 0
+#define UKV_CACHE_FP8 1
+
+/*
+ * Quantise rows into pages (write) or read them back in 16 bits (read), K and V in one launch.
+ *   k_new, v_new / k_out, v_out  rows [total, num_heads, head_dim] of `dtype`, last dimension contiguous; strides
+ *                       {K row, K head, V row, V head} in elements
+ *   cu_seqlens          int32 [batch + 1]: sequence b's rows are cu[b] .. cu[b + 1] - 1; NULL: max_chunk rows each
+ *   lens                int32 [batch]: the sequence holds lens[b] + lens_add tokens, its rows the last of them; NULL: its
+ *                       rows alone, from position 0. (read has no lens_add)
+ *   max_chunk           the longest sequence's rows; sizes the launch, longer ones take longer
+ * Position p of sequence b is slot p % 16 of page block_table[b, p / 16]. A row whose position lies outside
+ * the table or whose page lies outside [0, num_pages) is not written, and reads as zeros. Two rows of one
+ * call must not share a position. Replace core/scheduler.py:401-408 and core/pool.py:127-172 for this cache.
+ */
+int ukv_quant_kv_write(void* k, void* v, void* k_scale, void* v_scale, const int64_t* layer_strides, int num_pages,
+                       const void* k_new, const void* v_new, const int64_t* new_strides, const int32_t* block_table,
+                       int max_blocks, const int32_t* cu_seqlens, const int32_t* lens, int lens_add, int batch,
+                       int max_chunk, int num_heads, int head_dim, int format, int dtype, ukv_stream_t stream);
+int ukv_quant_kv_read(const void* k, const void* v, const void* k_scale, const void* v_scale,
+                      const int64_t* layer_strides, int num_pages, void* k_out, void* v_out, const int64_t* out_strides,
+                      const int32_t* block_table, int max_blocks, const int32_t* cu_seqlens, const int32_t* lens,
+                      int batch, int max_chunk, int num_heads, int head_dim, int format, int dtype, ukv_stream_t stream);
+
+/*
+ * ukv_page16_decode over the 8-bit cache: the same queries, table, lengths and result, K and V the values the
+ * cache holds. A key whose block reads as NaN makes NaN what attends to it; keys past the length and pages outside
+ * the pool have no part in the result. Workspace as for ukv_page16_decode (ukv_page16_workspace_bytes).
+ * Replaces core/page16_native.py:83-150 for this cache.
+ */
+int ukv_quant_decode(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale,
+                     const int64_t* layer_strides, int num_pages, const int32_t* block_table, const int32_t* seqlens,
+                     void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim, int n_rep, int max_blocks,
+                     const int64_t* q_strides, float softmax_scale, int format, int dtype, void* workspace,
+                     size_t workspace_bytes, ukv_stream_t stream);
+
+/*
+ * ukv_paged_prefill_parts over the 8-bit cache, without statistics: packed chunk queries, causal, bottom right
+ * aligned. Workspace as there (ukv_paged_prefill_workspace_bytes; without it the keys stay in one part).
+ * Replaces core/engine.py:1826-1854 for this cache.
+ */
+int ukv_quant_prefill(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale,
+                      const int64_t* layer_strides, int num_pages, const int32_t* block_table,
+                      const int32_t* cu_seqlens_q, const int32_t* kv_lens, void* out, int batch, int total_q,
+                      int max_chunk, int num_q_heads, int num_kv_heads, int head_dim, int n_rep, int max_blocks,
+                      const int64_t* q_strides, float softmax_scale, int format, int dtype, void* workspace,
+                      size_t workspace_bytes, ukv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

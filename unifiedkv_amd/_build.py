@@ -29,6 +29,7 @@ SOURCES = [
     "compact_plan.hip",
     "paged_prefill.hip",
     "snapkv_score.hip",
+    "quant_kv.hip",
 ]
 
 # Packed-FP32 VALU instructions are disabled for all device code.

@@ -19,6 +19,9 @@ LIB_PATH = PKG_DIR / "libukv.so"
 UKV_DTYPE_F16 = 0
 UKV_DTYPE_BF16 = 1
 
+UKV_CACHE_INT8 = 0
+UKV_CACHE_FP8 = 1
+
 UKV_OK = 0
 UKV_ERR_INVALID_ARGUMENT = -1
 UKV_ERR_EMPTY = -2
@@ -216,6 +219,43 @@ SIGNATURES = {
         _c_int,
         [_c_void_p, ctypes.c_int64, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p, ctypes.c_int64,
          _c_void_p],
+    ),
+    "ukv_quant_kv_write": (
+        _c_int,
+        [
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64p, _c_int,  # k v k_scale v_scale strides pages
+            _c_void_p, _c_void_p, _c_i64p,  # k_new v_new strides
+            _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,  # table max_blocks cu lens lens_add
+            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,  # batch max_chunk heads D format dtype stream
+        ],
+    ),
+    "ukv_quant_kv_read": (
+        _c_int,
+        [
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64p, _c_int,  # k v k_scale v_scale strides pages
+            _c_void_p, _c_void_p, _c_i64p,  # k_out v_out strides
+            _c_void_p, _c_int, _c_void_p, _c_void_p,  # table max_blocks cu lens
+            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,  # batch max_chunk heads D format dtype stream
+        ],
+    ),
+    "ukv_quant_decode": (
+        _c_int,
+        [
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64p, _c_int,  # q k v scales strides pages
+            _c_void_p, _c_void_p, _c_void_p,  # table seqlens out
+            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64p,  # batch Hq Hkv D n_rep max_blocks q strides
+            ctypes.c_float, _c_int, _c_int, _c_void_p, ctypes.c_size_t, _c_void_p,  # scale format dtype ws bytes stream
+        ],
+    ),
+    "ukv_quant_prefill": (
+        _c_int,
+        [
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64p, _c_int,  # q k v scales strides pages
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # table cu kv_lens out
+            _c_int, _c_int, _c_int,  # batch total_q max_chunk
+            _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64p,  # Hq Hkv D n_rep max_blocks q strides
+            ctypes.c_float, _c_int, _c_int, _c_void_p, ctypes.c_size_t, _c_void_p,  # scale format dtype ws bytes stream
+        ],
     ),
 }
 

@@ -42,6 +42,7 @@ import torch
 
 from . import _ext, page_ops
 from .page16_native import _current_stream as _stream
+from .pool import require_16bit_pool
 
 
 def selection_budget_blocks(L: int, *, block_size: int = 16, sink_len: int = 16, obs_len: int = 16,
@@ -316,6 +317,7 @@ def write_block_indexed_layer(pool, layer_id: int, block_ids: Sequence[int], K: 
     """core/scheduler.py:702-733 for one layer: whole source blocks of the dense raw K/V [H, L, D]
     into ``block_ids``, one launch. Returns False in the reference's bail-out cases (mismatched
     lengths, L not a multiple of the block, a source block outside [0, L/B))."""
+    require_16bit_pool(pool, "write_block_indexed_layer")
     B = int(pool.B)
     if not source_block_indices or len(source_block_indices) != len(block_ids):
         return False
@@ -344,6 +346,7 @@ def selected_writeback(pool, raw_by_layer: Sequence[Tuple[torch.Tensor, torch.Te
     freed again before the error propagates, as the reference's transaction does. A selection
     entry outside the middle blocks (a -1 pad of select_blocks, an index past the middle) raises
     ValueError before any page is taken (one host synchronisation for a device selection)."""
+    require_16bit_pool(pool, "selected_writeback")
     if len(raw_by_layer) != pool.num_layers:
         raise RuntimeError(f"selected_writeback_missing_raw layers={len(raw_by_layer)}")
     L = int(raw_by_layer[0][0].shape[1])
@@ -425,6 +428,7 @@ def compact_selected(pool, seq_page_lists: Sequence[Sequence[int]], seq_lens: Se
     page taken by this call is returned. Invalid input (a page outside the pool, a length beyond
     its pages or below its sink, a selection outside the middle) raises ValueError before any
     page is taken."""
+    require_16bit_pool(pool, "compact_selected")
     dev = pool.device
     layers = pool.num_layers
     results: List[List[int]] = []
@@ -497,6 +501,7 @@ def prune_window(pool, old_block_ids: Sequence[int], old_len: int, kept_blocks: 
     last block included) into them, then free the old ids in list order. kept_blocks are block
     indices into old_block_ids; the reference passes them sorted and unique, and so must the
     caller. Returns the new ids, or None when the pool cannot supply them (nothing changes)."""
+    require_16bit_pool(pool, "prune_window")
     B = int(pool.B)
     old = [int(x) for x in old_block_ids]
     kept = [int(b) for b in kept_blocks]

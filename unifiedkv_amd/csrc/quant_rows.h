@@ -1,0 +1,23 @@
+// The attention over the 8-bit cache for any head shape and alignment (quant_kv.hip), which the matrix-core
+// kernels' calls fall back on.
+#pragma once
+
+#include "quant_common.h"
+
+namespace ukv {
+
+struct QuantAttnArgs {
+  QuantLayer c;
+  const uint16_t* q;  // [rows][Hq][D], element strides q_st, q_sh
+  uint16_t* out;      // [rows][Hq][D] contiguous
+  int64_t q_st, q_sh;
+  const int32_t* bt;
+  const int32_t* cu;    // [B + 1] first query row of each sequence; null: row b is sequence b's one query
+  const int32_t* lens;  // [B] keys of each sequence, its queries' own included
+  int B, Hq, n_rep, D, max_blocks, max_chunk;
+  float scale;
+};
+
+int quant_rows_attention(const QuantAttnArgs& a, int rows, int dtype, int format, hipStream_t stream);
+
+}  // namespace ukv

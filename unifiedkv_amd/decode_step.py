@@ -37,7 +37,7 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from . import _ext, page16_native, page_ops
+from . import _ext, page16_native, page_ops, quant_kv
 from .pool import PagedKVPool, pack_block_table
 
 _TABLE_ALIGN = 64  # table width granularity in pages (1024 tokens)
@@ -84,7 +84,8 @@ class DecodeBatch:
 
     ``seq_page_lists[i]`` is sequence i's page list (its ``gpu_block_map``, shared by all
     layers) and ``seq_lens[i]`` its current length. The lists are owned by the batch from
-    here on (``page_lists`` returns them).
+    here on (``page_lists`` returns them). A ``quant_kv.QuantizedKVPool`` is taken like the 16-bit
+    one: its layers' appends quantise and its attention reads the 8-bit pages.
 
     Streams: the device table and lengths are written on the stream current at construction
     and at each ``begin_step`` and read on the stream current at each layer call; a caller that
@@ -122,6 +123,7 @@ class DecodeBatch:
             raise ValueError("a page appears in more than one sequence's list")
         self.on_pool_full = on_pool_full
         self.fused_append = bool(fused_append)
+        self._quant = getattr(pool, "cache_format", None) is not None
         pool.ensure_allocated()
         self.device = pool.device
         self.batch = len(self._lists)
@@ -208,8 +210,12 @@ class DecodeBatch:
         """Append the step's K/V rows of ``layer_id`` and attend (core/scheduler.py:401-418)."""
         if not self._open:
             raise RuntimeError("decode_step_not_open")
-        k_layer, v_layer = self.pool.k_cache[layer_id], self.pool.v_cache[layer_id]
         attn_lens = self._lens_dev[self._cur ^ 1]
+        if self._quant:  # (fused_append or not: the 8-bit append is a kernel of its own)
+            self.append(layer_id, k_new, v_new)
+            return quant_kv.decode_attention(q, self.pool.layer(layer_id), self._table, attn_lens,
+                                             softmax_scale=softmax_scale, n_rep=n_rep)
+        k_layer, v_layer = self.pool.k_cache[layer_id], self.pool.v_cache[layer_id]
         if self.fused_append:
             return page16_native.page16_decode_append_attention(
                 q, k_layer, v_layer, self._table, attn_lens, k_new, v_new, softmax_scale=softmax_scale, n_rep=n_rep)
@@ -222,6 +228,10 @@ class DecodeBatch:
         if not self._open:
             raise RuntimeError("decode_step_not_open")
         pool = self.pool
+        if self._quant:
+            quant_kv.append_kv(pool.layer(layer_id), pool._as_pool_rows(k_new), pool._as_pool_rows(v_new), self._table,
+                               self._lens_dev[self._cur])
+            return
         page_ops.kv_append(pool.k_cache[layer_id], pool.v_cache[layer_id], self._table, self._lens_dev[self._cur],
                            pool._as_pool_rows(k_new), pool._as_pool_rows(v_new), return_new_lens=False)
 
@@ -235,7 +245,8 @@ class DecodeBatch:
 
     def context(self) -> Dict[str, object]:
         """The dict ``prepare_page16_native_context`` returns (core/scheduler.py:1150-1160), for
-        callers that index it; every layer view shares the one device table."""
+        callers that index it; every layer view shares the one device table. (Not for a quantised pool, whose
+        layers have no 16-bit caches: its callers take ``pool.layer``.)"""
         views = {lid: {"k_cache": self.pool.k_cache[lid], "v_cache": self.pool.v_cache[lid],
                        "block_table": self._table} for lid in range(self.pool.num_layers)}
         return {

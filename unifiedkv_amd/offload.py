@@ -31,6 +31,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _ext, page_ops
+from .pool import require_16bit_pool
 
 ON_GPU, MIXED, ON_CPU = "ON_GPU", "MIXED", "ON_CPU"
 OFFLOAD_INFLIGHT, PREFETCH_INFLIGHT = "OFFLOAD_INFLIGHT", "PREFETCH_INFLIGHT"
@@ -100,6 +101,7 @@ class PinnedArena:
     """Pinned host page slots for every layer of a pool: K and V ``[layers, capacity, page]``."""
 
     def __init__(self, pool, capacity_pages: int):
+        require_16bit_pool(pool, "offload")
         self.capacity = int(capacity_pages)
         self.page_elems = pool.B * pool.num_kv_heads * pool.head_dim
         shape = (pool.num_layers, self.capacity, self.page_elems)
@@ -128,6 +130,7 @@ class SequenceOffloader:
 
     def __init__(self, pool, arena_pages: int, chunk_pages: int = 256,
                  offload_budget_blocks: Optional[int] = None, prefetch_budget_blocks: Optional[int] = None):
+        require_16bit_pool(pool, "offload")
         pool.ensure_allocated()
         self.pool = pool
         self.dev = pool.device

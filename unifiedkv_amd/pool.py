@@ -41,8 +41,16 @@ def pack_block_table(seq_block_ids_list: Sequence[Sequence[int]]) -> np.ndarray:
     return host
 
 
+def require_16bit_pool(pool, what: str) -> None:
+    """Raises for a pool of quantised pages (quant_kv.QuantizedKVPool), before anything is allocated or moved."""
+    if getattr(pool, "cache_format", None) is not None:
+        raise RuntimeError(f"quant_kv_shape_unsupported:{what}")
+
+
 class PagedKVPool:
     """Paged KV storage: k_cache / v_cache [num_layers, N_total, B, h_kv, d]; tables pad with 0."""
+
+    cache_format: Optional[str] = None  # a quantised pool's format; None: pages of ``dtype``
 
     def __init__(
         self,
@@ -71,8 +79,7 @@ class PagedKVPool:
             reserve = int(0.10 * total_gpu)
             available = total_gpu - model_used - reserve
             max_kv_mem = int(available * gpu_mem_frac)
-            bytes_per_block = 2 * num_layers * block_size * num_kv_heads * head_dim * 2
-            self.N_total = max(1, int(max_kv_mem / bytes_per_block))
+            self.N_total = max(1, int(max_kv_mem / self._bytes_per_block()))
         else:
             self.N_total = max(1, int(num_blocks))
 
@@ -94,6 +101,9 @@ class PagedKVPool:
         # The last id list token I/O uploaded (list, stream, device ids): callers pass the same
         # list once per layer.
         self._ids_cache: Optional[Tuple[List[int], int, torch.Tensor]] = None
+
+    def _bytes_per_block(self) -> int:
+        return 2 * self.num_layers * self.B * self.num_kv_heads * self.head_dim * 2
 
     # ------------------------------------------------------------------ storage
     @property

@@ -222,7 +222,9 @@ class PrefillPages:
     * ``end_chunk()`` commits the lengths.
 
     ``page_lists`` / ``seq_lens`` are what ``DecodeBatch``, ``snapkv.score_blocks`` and
-    ``compaction.compact`` take next; no dense copy of the prefill KV is ever made.
+    ``compaction.compact`` take next; no dense copy of the prefill KV is ever made. A
+    ``quant_kv.QuantizedKVPool`` is taken like the 16-bit pool, without ``obs_stats``: the chunk's K/V are
+    quantised into its pages, and the attention sees them as every later call will.
 
     Streams: the chunk's table and lengths are uploaded on the stream current at ``begin_chunk``
     and read on the stream current at each later call; a caller that moves to another stream
@@ -242,6 +244,11 @@ class PrefillPages:
             if len(ids) * pool.B < int(L):
                 raise ValueError("PrefillPages: a sequence has fewer pages than its length needs")
         pool.ensure_allocated()
+        self._quant = None
+        if getattr(pool, "cache_format", None) is not None:
+            from . import quant_kv  # (it takes this module's checks)
+
+            self._quant = quant_kv
         self.pool = pool
         self.dev = pool.device
         self._lists = [[int(x) for x in ids] for ids in page_lists]
@@ -318,6 +325,10 @@ class PrefillPages:
         if c["total"] == 0:
             return
         self._read_here(c)
+        if self._quant is not None:
+            self._quant.write_chunk_kv(pool.layer(layer_id), k_new, v_new, c["bt"], c["cu"], c["kv"],
+                                       max_chunk=c["max_chunk"])
+            return
         if (k_new.dtype != pool.dtype or v_new.dtype != pool.dtype or k_new.device != self.dev
                 or tuple(k_new.shape) != (c["total"], pool.num_kv_heads, pool.head_dim)
                 or k_new.stride() != v_new.stride() or k_new.stride(-1) != 1):
@@ -345,10 +356,17 @@ class PrefillPages:
         ``obs_stats``: this is the sequences' final chunk; also record layer ``layer_id``'s
         SnapKV normalisers of the last ``obs_len`` queries (see ``snapkv.ObsStats``)."""
         c = self._open()
+        if obs_stats is not None and self._quant is not None:
+            raise RuntimeError("quant_kv_shape_unsupported:obs_stats")
         if c["total"] == 0 and obs_stats is None:
             return torch.empty_like(q)
         self.write(layer_id, k_new, v_new)
         self._read_here(c)
+        if self._quant is not None:
+            lens = (c["lens"], [L + n for L, n in zip(self._lens, c["lens"])])
+            return self._quant.prefill_attention(q, self.pool.layer(layer_id), c["bt"], c["cu"], c["kv"],
+                                                 softmax_scale=softmax_scale, n_rep=n_rep, max_chunk=c["max_chunk"],
+                                                 host_lens=lens)
         host_lens = None
         if obs_stats is not None:
             host_lens = (c["lens"], [L + n for L, n in zip(self._lens, c["lens"])])

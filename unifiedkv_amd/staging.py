@@ -26,6 +26,7 @@ from typing import List, Sequence
 import torch
 
 from . import page_ops
+from .pool import require_16bit_pool
 
 
 @dataclass
@@ -45,6 +46,7 @@ class PageStager:
     """Chunked pool <-> pinned-host page mover on its own stream."""
 
     def __init__(self, pool, chunk_pages: int = 512):
+        require_16bit_pool(pool, "offload")
         self.pool = pool
         self.dev = pool.device
         self.chunk = int(chunk_pages)
