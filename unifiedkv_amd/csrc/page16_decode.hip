@@ -34,8 +34,10 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
-#include "ukv_common.h"
+#include "quant_common.h"
+#include "quant_rows.h"
 
 namespace ukv {
 
@@ -66,6 +68,17 @@ struct DecodeArgs {
   float scale;       // natural-log units (scalar kernel)
   float scale_log2;  // scale * log2(e) (split kernel)
 };
+
+// The 8-bit cache (QF: its format; kCache16: pages of the model's type): k and v are bytes, with strides in
+// bytes, and these their exponents.
+constexpr int kCache16 = -1;
+struct QuantDecodeArgs : DecodeArgs {
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
+};
+template <int QF> struct SplitArgs { typedef QuantDecodeArgs type; };
+template <> struct SplitArgs<kCache16> { typedef DecodeArgs type; };
 
 __device__ __forceinline__ int clamp_len(int L, int max_blocks) {
   const int cap = max_blocks * 16;
@@ -152,6 +165,9 @@ template <> struct PSplit<UKV_DTYPE_F16> {
 #ifndef UKV_PAGE16_WAVES
 #define UKV_PAGE16_WAVES 8
 #endif
+#ifndef UKV_QUANT_PIPE
+#define UKV_QUANT_PIPE 3
+#endif
 #ifndef UKV_PAGE16_MIN_WAVES_PER_EU
 #define UKV_PAGE16_MIN_WAVES_PER_EU 1
 #endif
@@ -169,6 +185,29 @@ __device__ __forceinline__ u32x2 ld8_stream(const uint16_t* p) {
 
 // V row fragment of one lane: DPL = D/16 consecutive dims of one token.
 template <int DPL> struct VRow { uint32_t w[DPL / 2]; };
+
+// A query row's B operand (this lane's eight dims of each step) from the model's type to fp16, times 2^-a
+// with a for the row's largest magnitude to land in [2^13, 2^14); returns 2^a. fp16 rows stay as they are.
+template <int DT, int STEPS> __device__ __forceinline__ float query_to_f16(u32x4 (&q)[STEPS]) {
+  if constexpr (DT == UKV_DTYPE_F16) return 1.f;
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m = __builtin_elementwise_max(m, as_u16x2(q[s][c] & 0x7fff7fffu));
+  int top = max((int)m[0], (int)m[1]) >> 7;  // the largest exponent field
+  top = max(top, __shfl_xor(top, 16));
+  top = max(top, __shfl_xor(top, 32));
+  const float down = __uint_as_float((uint32_t)min(267 - top, 254) << 23);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = q[s][c];
+      q[s][c] = pack_f16(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+    }
+  return top > 13 ? __uint_as_float((uint32_t)(top - 13) << 23) : 0x1p-127f;
+}
 
 template <int DPL>
 __device__ __forceinline__ void store_vrow(uint16_t* p, const VRow<DPL>& r) {
@@ -196,6 +235,41 @@ __device__ __forceinline__ void load_vrow(const uint16_t* p, VRow<DPL>& r) {
       r.w[4 * c + 2] = x[2];
       r.w[4 * c + 3] = x[3];
     }
+  }
+}
+
+// One lane's part of a page as loaded: dims DPL * i16 .. of tokens 4 * kg + t, and, of the 8-bit cache, those
+// tokens' exponents of the block the dims lie in (token t's in byte t).
+template <int DPL, int QF> struct PageRows {
+  struct Row { uint32_t w[DPL / 4]; };
+  Row k[4], v[4];
+  uint32_t ke, ve;
+};
+template <int DPL> struct PageRows<DPL, kCache16> { VRow<DPL> k[4], v[4]; };
+
+template <int DPL, class R> __device__ __forceinline__ void load_codes(const uint8_t* p, R& r) {
+  if constexpr (DPL == 4) {
+    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  } else if constexpr (DPL == 8) {
+    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+    r.w[0] = x[0];
+    r.w[1] = x[1];
+  } else {
+    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) r.w[c] = x[c];
+  }
+}
+
+// Codes -> fp16 values. An exponent byte of 255 is 2^128, infinity: zero codes make NaN of it, e4m3's are NaN.
+template <int DPL, int QF, class R>
+__device__ __forceinline__ void widen(const R& r, uint32_t exps, int t, VRow<DPL>& out) {
+  const float scale = __uint_as_float((exps >> (8 * t) & 255u) << 23);
+#pragma unroll
+  for (int c = 0; c < DPL / 4; ++c) {
+    const u32x2 x = quant_f16x4<QF>(r.w[c], scale);
+    out.w[2 * c] = x[0];
+    out.w[2 * c + 1] = x[1];
   }
 }
 
@@ -236,13 +310,23 @@ __device__ __forceinline__ void load_vrow(const uint16_t* p, VRow<DPL>& r) {
 // DIRECT (short tables): workgroup (b, g) takes the whole of sequence b for KV head g, its waves
 // sharing the pages as under SHARED, and writes the output itself: no partials, no second kernel, and
 // the table row is read beside the length instead of after it.
+//
+// QF: K and V are 8-bit codes (quant_common.h). A page's codes stay in the registers as loaded until the page is
+// reduced, then become fp16 values, which they are exactly, and go the way of an fp16 page; bf16 queries become fp16
+// too, moved by a power of two for each row that the scale takes back (28 binades below a row's largest value are
+// exact). Half the bytes a page: twice the pages in flight for the same cover of HBM's latency.
 enum SplitMode { kSplit = 0, kShared = 1, kDirect = 2 };
-template <int DT, int D, bool APPEND, int MODE>
-__global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PER_EU) page16_split_kernel(const DecodeArgs a) {
+template <int DT, int D, bool APPEND, int MODE, int QF = kCache16>
+__global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PER_EU)
+page16_split_kernel(const typename SplitArgs<QF>::type a) {
+  constexpr bool QUANT = QF != kCache16;
+  constexpr int MT = QUANT ? (int)UKV_DTYPE_F16 : DT;  // the type the matrix cores take
+  static_assert(!(QUANT && APPEND), "the 8-bit append is a kernel of its own");
   constexpr int STEPS = D / 32;  // QK k-steps of 32 dims
   constexpr int DPL = D / 16;    // V dims per lane = P.V output tiles
   constexpr float kTau = 8.f;
-  constexpr int kPipe = D > 128 ? 1 : 2;  // register sets (D=256 has no registers for a second page)
+  // register sets (D=256 has no registers for a second page)
+  constexpr int kPipe = D > 128 ? 1 : QUANT ? UKV_QUANT_PIPE : 2;
 
   const int lane = threadIdx.x & 63;
   const int wv = threadIdx.x >> 6;
@@ -338,7 +422,8 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
   const int n_here = min(a.n_rep, a.Hq - qh0);
   const bool live = i16 < n_here;
 
-  const uint16_t* kbase = a.k + (int64_t)(4 * kg) * a.k_st + (int64_t)g * a.k_sh + DPL * i16;
+  typedef std::conditional_t<QUANT, uint8_t, uint16_t> CacheElem;
+  const CacheElem* kbase = (const CacheElem*)a.k + (int64_t)(4 * kg) * a.k_st + (int64_t)g * a.k_sh + DPL * i16;
   // Wave-private LDS rows of the page's K (token-major): rows are loaded 4 tokens
   // x full width per instruction and read back in MFMA layout. The pitch of D + 16
   // elements (288 B at D = 128) keeps SQ_LDS_BANK_CONFLICT at 0 for the 16-row
@@ -349,7 +434,7 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
   // SHARED: the waves' partial rows and (m, l) of a segment.
   __shared__ __attribute__((aligned(16))) float part_lds[SHARED ? UKV_PAGE16_WAVES * 16 * D : 4];
   __shared__ float2 ml_lds[SHARED ? UKV_PAGE16_WAVES * 16 : 1];
-  const uint16_t* vbase = a.v + (int64_t)(4 * kg) * a.v_st + (int64_t)g * a.v_sh + DPL * i16;
+  const CacheElem* vbase = (const CacheElem*)a.v + (int64_t)(4 * kg) * a.v_st + (int64_t)g * a.v_sh + DPL * i16;
 
   // Per-segment state (one sequence's share of this workgroup's pages).
   int b = b_first;   // current sequence
@@ -366,6 +451,7 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
   VRow<DPL> vtok;      // APPEND: the new V row (lanes kg == tail_slot / 4)
 
   u32x4 qb[STEPS];   // B operand of QK^T: column i16 = q head qh0 + i16 (zero beyond n_here)
+  float q_scale = 0.f;  // QUANT: the scale of head i16's scores (log2 units), its row's power of two included
   float m_ref;       // running max of head i16 (log2 units)
   float lsum;        // this lane's share of that head's sum of weights
   f32x4 acc[DPL];
@@ -373,7 +459,8 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
   auto page_window = [&](int i0) {
     bid_win = i0 + lane < n_mine ? btrow[SHARED ? pa + sub + (i0 + lane) * subs : pa + i0 + lane] : 0;
   };
-  auto load_page = [&](int idx, VRow<DPL> (&kr)[4], VRow<DPL> (&vr)[4], int& nv) {
+  typedef PageRows<DPL, QF> Page;
+  auto load_page = [&](int idx, Page& pg, int& nv) {
     const int p = SHARED ? pa + sub + idx * subs : pa + idx;
     if (!DIRECT && idx != 0 && (idx & 63) == 0) page_window(idx);
     int bid = __builtin_amdgcn_readlane(bid_win, idx & 63);
@@ -382,12 +469,22 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
       if (p == tail_page) tail_pid = ok ? bid : -1;
     bid = ok ? bid : 0;
     nv = ok ? min(16, L - 16 * p) : 0;
-    const uint16_t* kp = kbase + (int64_t)bid * a.k_sp;
+    const CacheElem* kp = kbase + (int64_t)bid * a.k_sp;
+    const CacheElem* vp = vbase + (int64_t)bid * a.v_sp;
+    if constexpr (QUANT) {
+      const int64_t h = g, blk = DPL * i16 / kQuantBlock;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) load_vrow<DPL>(kp + (int64_t)t * a.k_st, kr[t]);
-    const uint16_t* vp = vbase + (int64_t)bid * a.v_sp;
+      for (int t = 0; t < 4; ++t) load_codes<DPL>(kp + (int64_t)t * a.k_st, pg.k[t]);
+      pg.ke = *reinterpret_cast<const uint32_t*>(a.ks + bid * a.ks_sp + h * a.ks_sh + blk * a.ks_sb + 4 * kg);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) load_vrow<DPL>(vp + (int64_t)t * a.v_st, vr[t]);
+      for (int t = 0; t < 4; ++t) load_codes<DPL>(vp + (int64_t)t * a.v_st, pg.v[t]);
+      pg.ve = *reinterpret_cast<const uint32_t*>(a.vs + bid * a.vs_sp + h * a.vs_sh + blk * a.vs_sb + 4 * kg);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) load_vrow<DPL>(kp + (int64_t)t * a.k_st, pg.k[t]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) load_vrow<DPL>(vp + (int64_t)t * a.v_st, pg.v[t]);
+    }
   };
 
   // APPEND: on the token's page, its slot gets the new rows (per-lane register selects).
@@ -411,10 +508,10 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
     for (int s = 0; s < STEPS; ++s) ka[s] = *reinterpret_cast<const u32x4*>(ks + i16 * KP + 8 * kg + 32 * s);
     f32x4 sacc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) sacc = mfma16x16x32<DT>(ka[s], qb[s], sacc);
+    for (int s = 0; s < STEPS; ++s) sacc = mfma16x16x32<MT>(ka[s], qb[s], sacc);
     float s2[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s2[r] = sacc[r] * a.scale_log2;
+    for (int r = 0; r < 4; ++r) s2[r] = sacc[r] * (QUANT ? q_scale : a.scale_log2);
     if (nv < 16) {  // last page of the sequence or an invalid page id
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -447,23 +544,22 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
       lsum += p[r];
     }
     u32x2 phi, plo;
-    PSplit<DT>::split(p, phi, plo);
+    PSplit<MT>::split(p, phi, plo);
 #pragma unroll
     for (int c = 0; c < DPL / 2; ++c) {
       const u32x2 blo = {__builtin_amdgcn_perm(vr[1].w[c], vr[0].w[c], 0x05040100u),
                          __builtin_amdgcn_perm(vr[3].w[c], vr[2].w[c], 0x05040100u)};
       const u32x2 bhi = {__builtin_amdgcn_perm(vr[1].w[c], vr[0].w[c], 0x07060302u),
                          __builtin_amdgcn_perm(vr[3].w[c], vr[2].w[c], 0x07060302u)};
-      acc[2 * c] = mfma16x16x16<DT>(phi, blo, acc[2 * c]);
-      acc[2 * c] = mfma16x16x16<DT>(plo, blo, acc[2 * c]);
-      acc[2 * c + 1] = mfma16x16x16<DT>(phi, bhi, acc[2 * c + 1]);
-      acc[2 * c + 1] = mfma16x16x16<DT>(plo, bhi, acc[2 * c + 1]);
+      acc[2 * c] = mfma16x16x16<MT>(phi, blo, acc[2 * c]);
+      acc[2 * c] = mfma16x16x16<MT>(plo, blo, acc[2 * c]);
+      acc[2 * c + 1] = mfma16x16x16<MT>(phi, bhi, acc[2 * c + 1]);
+      acc[2 * c + 1] = mfma16x16x16<MT>(plo, bhi, acc[2 * c + 1]);
     }
   };
 
-  constexpr float kUnscale = 1.f / PSplit<DT>::kScale;
-  VRow<DPL> kb[kPipe][4];
-  VRow<DPL> vb[kPipe][4];
+  constexpr float kUnscale = 1.f / PSplit<MT>::kScale;
+  Page pages[kPipe];
   int nvb[kPipe];
   int seg_start = s_first;  // global index of page 0 of sequence b
   int x = x0;
@@ -496,16 +592,26 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
       const uint16_t* qp = a.q + (int64_t)b * a.q_sb + (int64_t)(qh0 + (live ? i16 : 0)) * a.q_sh + 8 * kg;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) qb[s] = live ? ld16(qp + 32 * s) : u32x4{0u, 0u, 0u, 0u};
+      if constexpr (QUANT) q_scale = a.scale_log2 * query_to_f16<DT, STEPS>(qb);
     }
     m_ref = kNegFltMax;
     lsum = 0.f;
 #pragma unroll
     for (int e = 0; e < DPL; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto reduce = [&](int i, VRow<DPL> (&kr)[4], VRow<DPL> (&vr)[4], int nv) {
+    auto reduce = [&](int i, Page& pg, int nv) {
       if constexpr (APPEND)
-        if ((SHARED ? pa + sub + i * subs : pa + i) == tail_page) swap_in_token(kr, vr);
-      process_page(kr, vr, nv);
+        if ((SHARED ? pa + sub + i * subs : pa + i) == tail_page) swap_in_token(pg.k, pg.v);
+      if constexpr (QUANT) {
+        VRow<DPL> kr[4], vr[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) widen<DPL, QF>(pg.k[t], pg.ke, t, kr[t]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) widen<DPL, QF>(pg.v[t], pg.ve, t, vr[t]);
+        process_page(kr, vr, nv);
+      } else {
+        process_page(pg.k, pg.v, nv);
+      }
     };
     if constexpr (DIRECT) {
       // Page i + 1 is in flight while page i is reduced: every load of the loop is unconditional, so
@@ -514,35 +620,35 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PE
       // saturate HBM, are 2 % faster with that one).
       constexpr int B1 = kPipe - 1;
       if (n_mine > 0) {
-        load_page(0, kb[0], vb[0], nvb[0]);
+        load_page(0, pages[0], nvb[0]);
         int i = 0;
         for (; i + 2 < n_mine; i += 2) {
-          load_page(i + 1, kb[B1], vb[B1], nvb[B1]);
-          reduce(i, kb[0], vb[0], nvb[0]);
-          load_page(i + 2, kb[0], vb[0], nvb[0]);
-          reduce(i + 1, kb[B1], vb[B1], nvb[B1]);
+          load_page(i + 1, pages[B1], nvb[B1]);
+          reduce(i, pages[0], nvb[0]);
+          load_page(i + 2, pages[0], nvb[0]);
+          reduce(i + 1, pages[B1], nvb[B1]);
         }
         if (i + 1 < n_mine) {
-          load_page(i + 1, kb[B1], vb[B1], nvb[B1]);
-          reduce(i, kb[0], vb[0], nvb[0]);
-          reduce(i + 1, kb[B1], vb[B1], nvb[B1]);
+          load_page(i + 1, pages[B1], nvb[B1]);
+          reduce(i, pages[0], nvb[0]);
+          reduce(i + 1, pages[B1], nvb[B1]);
         } else {
-          reduce(i, kb[0], vb[0], nvb[0]);
+          reduce(i, pages[0], nvb[0]);
         }
       }
     } else {
       // Register sets in turn: the loads of page i + kPipe - 1 are issued before page i is reduced.
 #pragma unroll
       for (int i = 0; i < kPipe - 1; ++i)
-        if (i < n_mine) load_page(i, kb[i], vb[i], nvb[i]);
+        if (i < n_mine) load_page(i, pages[i], nvb[i]);
       for (int base = 0; base < n_mine; base += kPipe) {
 #pragma unroll
         for (int u = 0; u < kPipe; ++u) {
           const int i = base + u;
           if (i < n_mine) {
             const int nxt = (u + kPipe - 1) % kPipe;  // constant after unrolling
-            if (i + kPipe - 1 < n_mine) load_page(i + kPipe - 1, kb[nxt], vb[nxt], nvb[nxt]);
-            reduce(i, kb[u], vb[u], nvb[u]);
+            if (i + kPipe - 1 < n_mine) load_page(i + kPipe - 1, pages[nxt], nvb[nxt]);
+            reduce(i, pages[u], nvb[u]);
           }
         }
       }
@@ -914,35 +1020,35 @@ size_t workspace_report(int batch, int hq, int d, int max_blocks) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int DT, int D>
-void launch_split(const DecodeArgs& a, hipStream_t stream) {
+// (the split kernel of a cache and a mode, with and without the append)
+template <int DT, int D, int MODE, int QF>
+void launch_mode(const typename SplitArgs<QF>::type& a, dim3 grid, dim3 block, hipStream_t stream) {
+  if constexpr (QF == kCache16)
+    if (a.k_new) {
+      hipLaunchKernelGGL((page16_split_kernel<DT, D, true, MODE, QF>), grid, block, 0, stream, a);
+      return;
+    }
+  hipLaunchKernelGGL((page16_split_kernel<DT, D, false, MODE, QF>), grid, block, 0, stream, a);
+}
+
+template <int DT, int D, int QF>
+void launch_split(const typename SplitArgs<QF>::type& a, hipStream_t stream) {
   // Waves left over by the KV heads share the heads' pages (D = 256 has no LDS for their rows).
   if constexpr (D <= 128) {
     if (direct_shape(a.B, a.n_groups, a.n_rep, a.D, a.max_blocks)) {
-      const dim3 grid(a.B, a.n_groups), block(64 * UKV_PAGE16_WAVES);
-      if (a.k_new)
-        hipLaunchKernelGGL((page16_split_kernel<DT, D, true, kDirect>), grid, block, 0, stream, a);
-      else
-        hipLaunchKernelGGL((page16_split_kernel<DT, D, false, kDirect>), grid, block, 0, stream, a);
+      launch_mode<DT, D, kDirect, QF>(a, dim3(a.B, a.n_groups), dim3(64 * UKV_PAGE16_WAVES), stream);
       return;
     }
     if (a.n_groups <= UKV_PAGE16_WAVES / 2) {
-      DecodeArgs s = a;
+      auto s = a;
       for (s.subs = 2; 2 * s.subs * a.n_groups <= UKV_PAGE16_WAVES;) s.subs *= 2;
-      const dim3 grid(a.grid_wgs), block(64 * s.subs * a.n_groups);
-      if (a.k_new)
-        hipLaunchKernelGGL((page16_split_kernel<DT, D, true, kShared>), grid, block, 0, stream, s);
-      else
-        hipLaunchKernelGGL((page16_split_kernel<DT, D, false, kShared>), grid, block, 0, stream, s);
+      launch_mode<DT, D, kShared, QF>(s, dim3(a.grid_wgs), dim3(64 * s.subs * a.n_groups), stream);
       return;
     }
   }
   const int waves = std::min(UKV_PAGE16_WAVES, a.n_groups);
   const dim3 grid(a.grid_wgs, 1, (a.n_groups + waves - 1) / waves);
-  if (a.k_new)
-    hipLaunchKernelGGL((page16_split_kernel<DT, D, true, kSplit>), grid, dim3(64 * waves), 0, stream, a);
-  else
-    hipLaunchKernelGGL((page16_split_kernel<DT, D, false, kSplit>), grid, dim3(64 * waves), 0, stream, a);
+  launch_mode<DT, D, kSplit, QF>(a, grid, dim3(64 * waves), stream);
 }
 
 template <int DT>
@@ -963,13 +1069,13 @@ void launch_combine(const DecodeArgs& a, int dtype, hipStream_t stream) {
     launch_combine_dt<UKV_DTYPE_F16>(a, stream);
 }
 
-template <int DT>
-bool dispatch_split(const DecodeArgs& a, hipStream_t stream) {
+template <int DT, int QF = kCache16>
+bool dispatch_split(const typename SplitArgs<QF>::type& a, hipStream_t stream) {
   if (a.n_rep > 16) return false;
   switch (a.D) {
-    case 64: launch_split<DT, 64>(a, stream); return true;
-    case 128: launch_split<DT, 128>(a, stream); return true;
-    case 256: launch_split<DT, 256>(a, stream); return true;
+    case 64: launch_split<DT, 64, QF>(a, stream); return true;
+    case 128: launch_split<DT, 128, QF>(a, stream); return true;
+    case 256: launch_split<DT, 256, QF>(a, stream); return true;
     default: return false;
   }
 }
@@ -1088,6 +1194,72 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
 }
 
 }  // namespace
+
+// The decode over the 8-bit cache (arguments checked by the caller): the split kernel where the shape and the
+// alignment allow, else a workgroup for each (sequence, q head).
+int ukv::quant_decode(const QuantAttnArgs& x, int dtype, int format, void* workspace, size_t workspace_bytes,
+                      hipStream_t stream) {
+  const QuantLayer& c = x.c;
+  const int n_groups = (x.Hq + x.n_rep - 1) / x.n_rep;
+  const int64_t codes = c.k_sp | c.k_st | c.k_sh | c.v_sp | c.v_st | c.v_sh;
+  const int64_t exps = c.ks_sp | c.ks_sh | c.ks_sb | c.vs_sp | c.vs_sh | c.vs_sb;
+  auto aligned = [](const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  const unsigned wide = (unsigned)x.D / 16;  // bytes of a lane's dims
+  if (!((x.D == 64 || x.D == 128 || x.D == 256) && x.n_rep <= 16 && x.max_blocks > 0 && x.q_st % 8 == 0 &&
+        x.q_sh % 8 == 0 && (codes & (wide - 1)) == 0 && (exps & 3) == 0 && aligned16(x.q) && aligned16(x.out) &&
+        aligned(c.k, wide) && aligned(c.v, wide) && aligned(c.ks, 4) && aligned(c.vs, 4)))
+    return quant_rows_attention(x, x.B, dtype, format, stream);
+  const WorkspaceLayout w = workspace_layout(x.B, x.Hq, x.D, x.max_blocks);
+  if (!workspace || workspace_bytes < w.total || !aligned16(workspace)) return UKV_ERR_WORKSPACE;
+  QuantDecodeArgs a{};
+  a.q = x.q;
+  a.k = reinterpret_cast<const uint16_t*>(c.k);
+  a.v = reinterpret_cast<const uint16_t*>(c.v);
+  a.bt = x.bt;
+  a.lens = x.lens;
+  a.out = x.out;
+  a.q_sb = x.q_st;
+  a.q_sh = x.q_sh;
+  a.k_sp = c.k_sp;
+  a.k_st = c.k_st;
+  a.k_sh = c.k_sh;
+  a.v_sp = c.v_sp;
+  a.v_st = c.v_st;
+  a.v_sh = c.v_sh;
+  a.ks = c.ks;
+  a.vs = c.vs;
+  a.ks_sp = c.ks_sp;
+  a.ks_sh = c.ks_sh;
+  a.ks_sb = c.ks_sb;
+  a.vs_sp = c.vs_sp;
+  a.vs_sh = c.vs_sh;
+  a.vs_sb = c.vs_sb;
+  a.B = x.B;
+  a.Hq = x.Hq;
+  a.n_rep = x.n_rep;
+  a.n_groups = n_groups;
+  a.D = x.D;
+  a.max_blocks = x.max_blocks;
+  a.num_pages = c.num_pages;
+  a.scale = x.scale;
+  a.scale_log2 = x.scale * kLog2e;
+  char* ws = static_cast<char*>(workspace);
+  a.part_o = reinterpret_cast<float*>(ws + w.part_o_off);
+  a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml_off);
+  a.seq_start = reinterpret_cast<int32_t*>(ws + w.seq_off);
+  a.seq_pages = a.seq_start + x.B;
+  a.grid_wgs = launch_wgs(w.wgs, x.B, x.max_blocks, n_groups);
+  a.fixed_shares = env_wgs() > 0;
+  if (dtype == UKV_DTYPE_BF16)
+    format == UKV_CACHE_INT8 ? dispatch_split<UKV_DTYPE_BF16, UKV_CACHE_INT8>(a, stream)
+                             : dispatch_split<UKV_DTYPE_BF16, UKV_CACHE_FP8>(a, stream);
+  else
+    format == UKV_CACHE_INT8 ? dispatch_split<UKV_DTYPE_F16, UKV_CACHE_INT8>(a, stream)
+                             : dispatch_split<UKV_DTYPE_F16, UKV_CACHE_FP8>(a, stream);
+  if (hipGetLastError() != hipSuccess) return UKV_ERR_LAUNCH;
+  if (!direct_shape(x.B, n_groups, x.n_rep, x.D, x.max_blocks)) launch_combine(a, dtype, stream);
+  return hipGetLastError() == hipSuccess ? UKV_OK : UKV_ERR_LAUNCH;
+}
 
 extern "C" int ukv_page16_decode(const void* q, const void* k_cache, const void* v_cache,
                                  const int32_t* block_table, const int32_t* seqlens, void* out, int batch,

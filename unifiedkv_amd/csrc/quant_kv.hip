@@ -412,9 +412,7 @@ extern "C" int ukv_quant_decode(const void* q, const void* k, const void* v, con
                                 batch, batch, 1, num_q_heads, num_kv_heads, head_dim, n_rep, max_blocks, q_strides,
                                 softmax_scale, format, dtype, a);
   if (rc != UKV_OK) return rc;
-  (void)workspace;
-  (void)workspace_bytes;
-  return quant_rows_attention(a, batch, dtype, format, reinterpret_cast<hipStream_t>(stream));
+  return quant_decode(a, dtype, format, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int ukv_quant_prefill(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale,

@@ -18,6 +18,10 @@ struct QuantAttnArgs {
   float scale;
 };
 
+// page16_decode.hip; the workspace is ukv_page16_workspace_bytes().
+int quant_decode(const QuantAttnArgs& a, int dtype, int format, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream);
+
 int quant_rows_attention(const QuantAttnArgs& a, int rows, int dtype, int format, hipStream_t stream);
 
 }  // namespace ukv
