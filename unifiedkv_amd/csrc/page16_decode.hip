@@ -71,7 +71,6 @@ struct DecodeArgs {
 
 // The 8-bit cache (QF: its format; kCache16: pages of the model's type): k and v are bytes, with strides in
 // bytes, and these their exponents.
-constexpr int kCache16 = -1;
 struct QuantDecodeArgs : DecodeArgs {
   const uint8_t* ks;
   const uint8_t* vs;
@@ -185,29 +184,6 @@ __device__ __forceinline__ u32x2 ld8_stream(const uint16_t* p) {
 
 // V row fragment of one lane: DPL = D/16 consecutive dims of one token.
 template <int DPL> struct VRow { uint32_t w[DPL / 2]; };
-
-// A query row's B operand (this lane's eight dims of each step) from the model's type to fp16, times 2^-a
-// with a for the row's largest magnitude to land in [2^13, 2^14); returns 2^a. fp16 rows stay as they are.
-template <int DT, int STEPS> __device__ __forceinline__ float query_to_f16(u32x4 (&q)[STEPS]) {
-  if constexpr (DT == UKV_DTYPE_F16) return 1.f;
-  u16x2 m = {0, 0};
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) m = __builtin_elementwise_max(m, as_u16x2(q[s][c] & 0x7fff7fffu));
-  int top = max((int)m[0], (int)m[1]) >> 7;  // the largest exponent field
-  top = max(top, __shfl_xor(top, 16));
-  top = max(top, __shfl_xor(top, 32));
-  const float down = __uint_as_float((uint32_t)min(267 - top, 254) << 23);
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w = q[s][c];
-      q[s][c] = pack_f16(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
-    }
-  return top > 13 ? __uint_as_float((uint32_t)(top - 13) << 23) : 0x1p-127f;
-}
 
 template <int DPL>
 __device__ __forceinline__ void store_vrow(uint16_t* p, const VRow<DPL>& r) {
@@ -592,7 +568,14 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
       const uint16_t* qp = a.q + (int64_t)b * a.q_sb + (int64_t)(qh0 + (live ? i16 : 0)) * a.q_sh + 8 * kg;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) qb[s] = live ? ld16(qp + 32 * s) : u32x4{0u, 0u, 0u, 0u};
-      if constexpr (QUANT) q_scale = a.scale_log2 * query_to_f16<DT, STEPS>(qb);
+      if constexpr (QUANT) {
+        q_scale = a.scale_log2;
+        if constexpr (DT == UKV_DTYPE_BF16) {
+          const int top = query_top<STEPS>(qb);
+          query_to_f16<STEPS>(qb, top);
+          q_scale *= query_scale(top);
+        }
+      }
     }
     m_ref = kNegFltMax;
     lsum = 0.f;

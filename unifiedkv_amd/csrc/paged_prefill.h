@@ -56,14 +56,23 @@ struct PrefillArgs {
   int sink, obs;
 };
 
+// The 8-bit cache (QF: its format): k and v are bytes, with strides in bytes, and these their exponents.
+struct QuantPrefillArgs : PrefillArgs {
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
+};
+template <int QF> struct TileArgs { typedef QuantPrefillArgs type; };
+template <> struct TileArgs<kCache16> { typedef PrefillArgs type; };
+
 // paged_prefill_kernel's argument (its only one, at the start of the kernel's argument segment), read again
 // behind a barrier to the compiler: the fields that only a block's rows need at the end would otherwise be loaded
 // at the start and held through the tiles, where the scalar registers they spill cost a v_readlane each (16 a tile in
 // the parts' instance for three column blocks, 150 instructions of it against 128).
-__device__ __forceinline__ const PrefillArgs& args_again() {
-  auto* p = (const __attribute__((address_space(4))) PrefillArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+template <class Args> __device__ __forceinline__ const Args& args_again() {
+  auto* p = (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
-  return *(const PrefillArgs*)p;
+  return *(const Args*)p;
 }
 
 __device__ __forceinline__ int kv_len_of(const PrefillArgs& a, int b) {
@@ -87,6 +96,18 @@ __device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t w) {
 // loaded registers follow the wait.
 __device__ __forceinline__ void gload16(u32x4& r, const void* p) {
   asm volatile("global_load_dwordx4 %0, %1, off" : "=&v"(r) : "v"(p));
+}
+__device__ __forceinline__ void gload8(u32x2& r, const void* p) {
+  asm volatile("global_load_dwordx2 %0, %1, off" : "=&v"(r) : "v"(p));
+}
+__device__ __forceinline__ void gload_u8(uint32_t& r, const void* p) {
+  asm volatile("global_load_ubyte %0, %1, off" : "=&v"(r) : "v"(p));
+}
+template <int N> __device__ __forceinline__ void vm_wait(u32x2& x, uint32_t& e) {
+  asm volatile("s_waitcnt vmcnt(%2)" : "+v"(x), "+v"(e) : "n"(N));
+}
+template <int N> __device__ __forceinline__ void vm_wait(u32x2& x, u32x2& y, uint32_t& e, uint32_t& f) {
+  asm volatile("s_waitcnt vmcnt(%4)" : "+v"(x), "+v"(y), "+v"(e), "+v"(f) : "n"(N));
 }
 template <int N> __device__ __forceinline__ void vm_wait(u32x4& x) {
   asm volatile("s_waitcnt vmcnt(%1)" : "+v"(x) : "n"(N));
@@ -198,6 +219,62 @@ __device__ void prefill_cols_fp32(const PrefillArgs& a, int b, int g, int q_begi
   }
 }
 
+// The same over the 8-bit cache, for a workgroup whose visible or masked values hold a NaN (zero weights make NaN of
+// it).
+template <int DT, int D, int QF>
+__device__ void prefill_cols_fp32(const QuantPrefillArgs& a, int b, int g, int q_begin, int C, int P0, int Lk, int c0,
+                                  int n_cols, int wv, int nwaves, int lane, int part, int key_a, int key_b) {
+  constexpr int W = D / 64;  // dims per lane
+  const int32_t* btrow = a.bt + (int64_t)b * a.max_blocks;
+  const int64_t blk = W * lane / kQuantBlock;
+  for (int c = c0 + wv; c < c0 + n_cols; c += nwaves) {
+    if (c < 0) continue;
+    const int qi = c / a.n_rep;
+    const int h = g * a.n_rep + c % a.n_rep;
+    if (qi >= C || h >= a.Hq) continue;
+    const int L = min(key_b, max(0, min(Lk, P0 + qi + 1)));
+    const uint16_t* qrow = a.q + (int64_t)(q_begin + qi) * a.q_st + (int64_t)h * a.q_sh + W * lane;
+    float q[W], acc[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      q[w] = Elem<DT>::one(qrow[w]);
+      acc[w] = 0.f;
+    }
+    float m = kNegFltMax, l = 0.f;
+    for (int key = key_a; key < L; ++key) {
+      const int id = btrow[key >> 4];
+      if ((unsigned)id >= (unsigned)a.num_pages) continue;
+      const int64_t slot = key & 15;
+      const uint8_t* kr = (const uint8_t*)a.k + id * a.k_sp + slot * a.k_st + g * a.k_sh + W * lane;
+      const uint8_t* vr = (const uint8_t*)a.v + id * a.v_sp + slot * a.v_st + g * a.v_sh + W * lane;
+      const float ke = quant_scale(a.ks[id * a.ks_sp + g * a.ks_sh + blk * a.ks_sb + slot]);
+      const float ve = quant_scale(a.vs[id * a.vs_sp + g * a.vs_sh + blk * a.vs_sb + slot]);
+      float dot = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) dot += q[w] * quant_one<QF>(kr[w], ke);
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off);
+      const float sc = dot * a.scale;
+      const float mn = fmaxf(m, sc);
+      const float alpha = expf(m - mn), pk = expf(sc - mn);
+      l = l * alpha + pk;
+#pragma unroll
+      for (int w = 0; w < W; ++w) acc[w] = acc[w] * alpha + pk * quant_one<QF>(vr[w], ve);
+      m = mn;
+    }
+    if (part >= 0) {
+      const int64_t row = ((int64_t)part * a.total_q + q_begin + qi) * a.Hq + h;
+#pragma unroll
+      for (int w = 0; w < W; ++w) a.part_o[row * D + W * lane + w] = acc[w];
+      if (lane == 0) a.part_ml[row] = make_float2(m * kLog2e, l);
+      continue;
+    }
+    uint16_t* orow = a.out + ((int64_t)(q_begin + qi) * a.Hq + h) * D + W * lane;
+#pragma unroll
+    for (int w = 0; w < W; ++w) orow[w] = Elem<DT>::from_float(acc[w] / l);
+  }
+}
+
 // Flags (y = 1) the observation rows among queries lo .. hi - 1 of sequence b's chunk (C
 // queries), q heads of KV group g, for the scoring pass to recompute from the keys.
 template <int WAVES>
@@ -260,9 +337,13 @@ template <> struct PrefillSplit<UKV_DTYPE_F16> {
 // softmax denominator l (the sum of the rounded weights 2^(s * scale * log2e - m) over every key the
 // query sees; FINE: with its lift, taken off m) into obs_stats[b * stats_seq_stride + h * obs + i],
 // for obs_rows_finish_kernel.
-template <int DT, int D, int WAVES, int CB, bool FINE, bool PARTS>
-__device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, const int g, const int c0,
-                                             const int part, const int np, PrefillLds<D>& lds) {
+//   QF     the pages are 8-bit codes: a thread's chunk is eight codes and their exponent byte, which its store
+//          makes the values that they are exactly, K in the queries' type, V in that of P.V's operands. From LDS on
+//          the tile is a 16-bit pool's.
+template <int DT, int D, int WAVES, int CB, bool FINE, bool PARTS, int QF>
+__device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& a, const int b, const int g,
+                                             const int c0, const int part, const int np, PrefillLds<D>& lds) {
+  constexpr bool QUANT = QF != kCache16;
   constexpr int STEPS = D / 32;
   constexpr int NE = D / 16;  // output tiles of 16 dims
   constexpr int NT = 64 * WAVES;
@@ -275,7 +356,7 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
   constexpr int PVT = FINE ? DT : (int)UKV_DTYPE_F16;  // type of the P.V operands
   constexpr float kTau = 8.f;
   constexpr float kLift = FINE ? PrefillSplit<DT>::kLift : 0.f;
-  constexpr bool kConvert = DT == UKV_DTYPE_BF16 && !FINE;  // the loader converts V to fp16
+  constexpr bool kConvert = DT == UKV_DTYPE_BF16 && !FINE && !QUANT;  // the loader converts V to fp16
   static_assert(HALF || TK * CH == NT, "loader mapping");
   auto& k_s = lds.k_s;
   auto& v_s = lds.v_s;
@@ -378,6 +459,23 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
   const uint16_t* kbase = half_v ? a.v : a.k;
   const uint32_t k_sp = (uint32_t)(half_v ? a.v_sp : a.k_sp);
   u32x4 rk0, rv0, rk1, rv1;
+  // QUANT: a chunk of K and V as codes and their exponent bytes
+  struct Codes {
+    u32x2 k, v;
+    uint32_t ke, ve;
+  };
+  Codes r0, r1;
+  const uint8_t *ebase = nullptr, *vebase = nullptr;
+  uint32_t eoff = 0, veoff = 0, e_sp = 0, ve_sp = 0;
+  if constexpr (QUANT) {
+    const uint32_t blk = lds_ch / (kQuantBlock / 8);
+    ebase = half_v ? a.vs : a.ks;
+    e_sp = (uint32_t)(half_v ? a.vs_sp : a.ks_sp);
+    eoff = (uint32_t)(g * (half_v ? a.vs_sh : a.ks_sh) + blk * (half_v ? a.vs_sb : a.ks_sb) + tok);
+    vebase = a.vs;
+    ve_sp = (uint32_t)a.vs_sp;
+    veoff = (uint32_t)(g * a.vs_sh + blk * a.vs_sb + tok);
+  }
   // the page of this thread's chunk among a tile's two (rows 0-15 and 16-31); wave-uniform
   auto chunk_page = [&](const int (&ids)[PPT]) -> int {
     return __builtin_amdgcn_readfirstlane(idx / (16 * CH)) ? ids[1] : ids[0];
@@ -388,6 +486,16 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
     const uint32_t pg = page_ok(id) ? (uint32_t)id : 0u;
     gload16(rk, kbase + (uint64_t)pg * k_sp + koff);
     if constexpr (!HALF) gload16(rv, a.v + (uint64_t)pg * (uint32_t)a.v_sp + voff);
+  };
+  auto issue_codes = [&](const int (&ids)[PPT], Codes& r) {
+    const int id = chunk_page(ids);
+    const uint32_t pg = page_ok(id) ? (uint32_t)id : 0u;
+    gload8(r.k, (const uint8_t*)kbase + (uint64_t)pg * k_sp + koff);
+    gload_u8(r.ke, ebase + (uint64_t)pg * e_sp + eoff);
+    if constexpr (!HALF) {
+      gload8(r.v, (const uint8_t*)a.v + (uint64_t)pg * (uint32_t)a.v_sp + voff);
+      gload_u8(r.ve, vebase + (uint64_t)pg * ve_sp + veoff);
+    }
   };
   // The largest and the smallest fp16 V value this thread stored, over every tile (three-input
   // packed maximum / minimum, which carry a NaN through): checked once after the loop for an
@@ -430,6 +538,36 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
     *reinterpret_cast<u32x4*>(&k_s[slot][lds_row][8 * lds_ch]) = rk;
     *reinterpret_cast<u32x4*>(&v_s[slot][lds_row][8 * lds_ch]) = v;
   };
+  auto store_codes = [&](int u, int slot, const int (&ids)[PPT], Codes& r) {
+    const bool full = page_ok(ids[0]) && page_ok(ids[1]) && TK * (u + 1) <= Lk;
+    if constexpr (HALF) vm_wait<2>(r.k, r.ke);  // the other set's loads were issued after this one's
+    else vm_wait<4>(r.k, r.v, r.ke, r.ve);
+    auto clear_junk = [&](u32x2& codes, uint32_t& exps) {
+      if (!full) {
+        const bool ok = page_ok(chunk_page(ids)) && TK * u + lds_row < Lk;
+        codes[0] = ok ? codes[0] : 0u;
+        codes[1] = ok ? codes[1] : 0u;
+        exps = ok ? exps : 0u;
+      }
+    };
+    auto widen = [&](const u32x2& codes, uint32_t exps, auto type) -> u32x4 {
+      constexpr int F = QUANT ? QF : UKV_CACHE_INT8, T = decltype(type)::value;
+      const float scale = __uint_as_float(exps << 23);  // (255: infinity; times zero codes, or e4m3's NaN, is NaN)
+      const u32x2 lo = quant_elems4<F, T>(codes[0], scale), hi = quant_elems4<F, T>(codes[1], scale);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    std::integral_constant<int, DT> k_type;
+    std::integral_constant<int, PVT> v_type;
+    if constexpr (HALF) {
+      clear_junk(r.k, r.ke);
+      uint16_t* dst = half_v ? &v_s[slot][lds_row][8 * lds_ch] : &k_s[slot][lds_row][8 * lds_ch];
+      *reinterpret_cast<u32x4*>(dst) = widen(r.k, r.ke, k_type);
+    } else {
+      clear_junk(r.v, r.ve);
+      *reinterpret_cast<u32x4*>(&k_s[slot][lds_row][8 * lds_ch]) = widen(r.k, r.ke, k_type);
+      *reinterpret_cast<u32x4*>(&v_s[slot][lds_row][8 * lds_ch]) = widen(r.v, r.ve, v_type);
+    }
+  };
 
   // Page ids of tiles t .. t+3 (t_id[j] = tile t + j) and of tile t+4.
   int t_id[4][PPT], id_n[PPT];
@@ -442,12 +580,21 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
   // Prologue: tiles 0 and 1 into the ring, tiles 2 and 3 in flight. Loads are issued
   // unconditionally (tiles past the end read page 0 and are never used) so
   // that every wait is on loads of a fixed age: vmcnt(2) on the older set.
-  issue(t_id[0], rk0, rv0);
-  issue(t_id[1], rk1, rv1);
-  store(0, 0, t_id[0], rk0, rv0);
-  issue(t_id[2], rk0, rv0);
-  store(1, 1, t_id[1], rk1, rv1);
-  issue(t_id[3], rk1, rv1);
+  if constexpr (QUANT) {
+    issue_codes(t_id[0], r0);
+    issue_codes(t_id[1], r1);
+    store_codes(0, 0, t_id[0], r0);
+    issue_codes(t_id[2], r0);
+    store_codes(1, 1, t_id[1], r1);
+    issue_codes(t_id[3], r1);
+  } else {
+    issue(t_id[0], rk0, rv0);
+    issue(t_id[1], rk1, rv1);
+    store(0, 0, t_id[0], rk0, rv0);
+    issue(t_id[2], rk0, rv0);
+    store(1, 1, t_id[1], rk1, rv1);
+    issue(t_id[3], rk1, rv1);
+  }
   tile_ids(4, id_n);
   // Retire every load issued so far (q columns, tiles 2 and 3) once, so that
   // no wait for them is left inside the loop.
@@ -630,10 +777,15 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
     constexpr int Q = decltype(phase)::value;  // t % 4: the ring slot of tile t
     constexpr int P = Q & 1;                   // register set of tile t+2
     // (a slot written past the last tile is never read)
-    if constexpr (P == 0) store(t + 2, (Q + 2) & 3, t_id[2], rk0, rv0);
-    else store(t + 2, (Q + 2) & 3, t_id[2], rk1, rv1);
-    if constexpr (P == 0) issue(id_n, rk0, rv0);
-    else issue(id_n, rk1, rv1);
+    if constexpr (QUANT) {
+      store_codes(t + 2, (Q + 2) & 3, t_id[2], P == 0 ? r0 : r1);
+      issue_codes(id_n, P == 0 ? r0 : r1);
+    } else {
+      if constexpr (P == 0) store(t + 2, (Q + 2) & 3, t_id[2], rk0, rv0);
+      else store(t + 2, (Q + 2) & 3, t_id[2], rk1, rv1);
+      if constexpr (P == 0) issue(id_n, rk0, rv0);
+      else issue(id_n, rk1, rv1);
+    }
     do_compute(t, Q);
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
@@ -656,14 +808,24 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
   else run([](int, int) {});
   // Loads of tiles past the end are still in flight: retire them while their
   // registers are still held, so that nothing else is placed in them first.
-  vm_wait<0>(rk0);
-  vm_wait<0>(rk1);
-  if constexpr (!HALF) {
-    vm_wait<0>(rv0);
-    vm_wait<0>(rv1);
+  if constexpr (QUANT) {
+    vm_wait<0>(r0.k, r0.ke);
+    vm_wait<0>(r1.k, r1.ke);
+    if constexpr (!HALF) {
+      vm_wait<0>(r0.v, r0.ve);
+      vm_wait<0>(r1.v, r1.ve);
+    }
+  } else {
+    vm_wait<0>(rk0);
+    vm_wait<0>(rk1);
+    if constexpr (!HALF) {
+      vm_wait<0>(rv0);
+      vm_wait<0>(rv1);
+    }
   }
 
-  const PrefillArgs& e = PARTS ? args_again() : a;
+  // (QUANT: where holding them left no register for the scalar spills; in the other instances reading them again did)
+  const auto& e = PARTS || (QUANT && D == 128 && DT == UKV_DTYPE_BF16) ? args_again<typename TileArgs<QF>::type>() : a;
   // A V the matrix cores got wrong anywhere in this workgroup's keys: its columns again on the fp32
   // fallback.
   bool redo_mine = false;
@@ -673,8 +835,9 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
                                                 as_u16x2(__builtin_bit_cast(uint32_t, vmin) & 0x7fff7fffu));
     redo_mine = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(mag, u16x2{0x7BFF, 0x7BFF})) != 0u;
   }
-  if constexpr (FINE) {
-    // found from the accumulators: one that is not finite times zero is NaN
+  if constexpr (FINE || QUANT) {
+    // found from the accumulators: one that is not finite times zero is NaN (QUANT: the NaN of a key that a row does
+    // not see is not its own)
     float z = 0.f;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)
@@ -684,11 +847,15 @@ __device__ __forceinline__ void prefill_tile(const PrefillArgs& a, const int b, 
         for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o[cb][d][r], 0.f, z);
     redo_mine = z != 0.f;
   }
-  if constexpr (kConvert || FINE) {
+  if constexpr (kConvert || FINE || QUANT) {
     if (__syncthreads_or(redo_mine)) {
       if (!in_parts) flag_obs_rows<WAVES>(e, b, g, C, max(q0, 0), min(C, q1));  // (none without statistics)
-      prefill_cols_fp32<DT, D>(e, b, g, q_begin, C, P0 + key_a, Lk + key_a, c0, WAVES * CB * 16, wv, WAVES, lane,
-                               in_parts ? part : -1, key_a, key_a + kend);
+      if constexpr (QUANT)
+        prefill_cols_fp32<DT, D, QF>(e, b, g, q_begin, C, P0 + key_a, Lk + key_a, c0, WAVES * CB * 16, wv, WAVES, lane,
+                                     in_parts ? part : -1, key_a, key_a + kend);
+      else
+        prefill_cols_fp32<DT, D>(e, b, g, q_begin, C, P0 + key_a, Lk + key_a, c0, WAVES * CB * 16, wv, WAVES, lane,
+                                 in_parts ? part : -1, key_a, key_a + kend);
       return;
     }
   }
@@ -881,9 +1048,9 @@ __device__ __forceinline__ void xcd_range(int total, int xcd, int& start, int& e
 // parts, its workgroups past the items exiting at the end: 8 x 512 queries behind 4000 tokens in a 2048-page
 // table 292 us, 380 in the order of parts, 284 in a launch without parts. Looking for one costs a launch
 // in parts of several sequences a round of loads, ~1.3 us.
-template <int DT, int D, int WAVES, bool FINE, bool PARTS>
+template <int DT, int D, int WAVES, bool FINE, bool PARTS, int QF = kCache16>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
-paged_prefill_kernel(const PrefillArgs a) {
+paged_prefill_kernel(const typename TileArgs<QF>::type a) {
   __shared__ PrefillLds<D> lds;
   constexpr int CB3 = wide_blocks(FINE), CB2 = CB3 - 1;
   int n3 = a.n3, n2 = a.n2;
@@ -941,9 +1108,9 @@ paged_prefill_kernel(const PrefillArgs a) {
   }
   const int cols = C * a.n_rep;
   if (j < n3)
-    prefill_tile<DT, D, WAVES, CB3, FINE, PARTS>(a, b, g, cols - w3 * (j + 1), part, np, lds);
+    prefill_tile<DT, D, WAVES, CB3, FINE, PARTS, QF>(a, b, g, cols - w3 * (j + 1), part, np, lds);
   else
-    prefill_tile<DT, D, WAVES, CB2, FINE, PARTS>(a, b, g, cols - w3 * n3 - w2 * (j - n3 + 1), part, np, lds);
+    prefill_tile<DT, D, WAVES, CB2, FINE, PARTS, QF>(a, b, g, cols - w3 * n3 - w2 * (j - n3 + 1), part, np, lds);
 }
 
 namespace {
@@ -1000,29 +1167,59 @@ size_t part_bytes(int parts, int64_t rows, int head_dim) {
 // Partials above this are not worth their traffic: the launch is large enough without parts.
 constexpr size_t kMaxPartBytes = size_t(512) << 20;
 
+// The call's block plan, key parts and partials into `a`, whose other fields are set; returns the tiled launch's
+// workgroups. The caller sizes the workspace by the same plan; a smaller one runs without parts.
+int64_t plan_launch(PrefillArgs& a, int total_q, void* workspace, size_t workspace_bytes) {
+  const int64_t pairs = (int64_t)a.n_groups * a.B, rows = (int64_t)total_q * a.Hq;
+  BlockPlan plan = plan_for(a.B, rows, a.max_chunk, a.n_groups, a.D, a.n_rep, a.max_blocks, workspace != nullptr);
+  if (plan.parts > 1 && (part_bytes(plan.parts, rows, a.D) > workspace_bytes || (rows + 7) / 8 > INT32_MAX ||
+                         (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+    plan = plan_for(a.B, rows, a.max_chunk, a.n_groups, a.D, a.n_rep, a.max_blocks, false);
+  a.n3 = plan.n3;
+  a.n2 = plan.n2;
+  a.n_parts = plan.parts;
+  a.part_tiles = plan.part_tiles;
+  a.whole3 = plan.whole3;
+  a.whole2 = plan.whole2;
+  // No more keys than twice the chunk's: the blocks' key counts differ by a factor of two or more, and
+  // every pair's longest blocks go first. (With a long prefix they are alike, and the blocks of one
+  // pair stay together for their XCD's L2.)
+  a.by_block = (int64_t)a.max_blocks * 16 <= 2 * (int64_t)a.max_chunk;
+  a.total_q = total_q;
+  if (plan.parts > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + part_o_bytes(plan.parts, rows, a.D));
+  }
+  // Parts: eight times what an XCD runs at most. (Two parts' items hold a pair's whole blocks: narrow ones are
+  // at least half as wide as wide ones.)
+  const int64_t items = pairs * (a.n3 + a.n2);
+  return plan.parts > 1 ? 8 * ((items * plan.parts + 7) / 8) : items;
+}
+
 constexpr int kMergeWgs = 2048;
 
-template <int DT, int D, bool FINE, bool PARTS>
-void launch_tiled(const PrefillArgs& a, unsigned tile_wgs, hipStream_t stream) {
+template <int DT, int D, bool FINE, bool PARTS, int QF>
+void launch_tiled(const typename TileArgs<QF>::type& a, unsigned tile_wgs, hipStream_t stream) {
   constexpr int W = UKV_PREFILL_WAVES;
-  hipLaunchKernelGGL((paged_prefill_kernel<DT, D, W, FINE, PARTS>), dim3(tile_wgs), dim3(64 * W), 0, stream, a);
+  hipLaunchKernelGGL((paged_prefill_kernel<DT, D, W, FINE, PARTS, QF>), dim3(tile_wgs), dim3(64 * W), 0, stream, a);
   if constexpr (PARTS) {
     constexpr int ROWS = 256 / (D / 4);
     const int64_t rows = (int64_t)a.total_q * a.Hq;
     // (eight workgroups a CU at once; rows beyond them are taken in turn)
     const int64_t wgs = std::min<int64_t>((rows + ROWS - 1) / ROWS, kMergeWgs);
-    hipLaunchKernelGGL((prefill_combine_kernel<DT, D>), dim3((unsigned)wgs), dim3(256), 0, stream, a);
+    const PrefillArgs& merge = a;
+    hipLaunchKernelGGL((prefill_combine_kernel<DT, D>), dim3((unsigned)wgs), dim3(256), 0, stream, merge);
   }
 }
 
-template <int DT, bool PARTS>
-void launch_tiled_dt(const PrefillArgs& a, bool fine, unsigned wgs, hipStream_t stream) {
+template <int DT, bool PARTS, int QF = kCache16>
+void launch_tiled_dt(const typename TileArgs<QF>::type& a, bool fine, unsigned wgs, hipStream_t stream) {
   if (a.D == 64)
-    launch_tiled<DT, 64, true, PARTS>(a, wgs, stream);
+    launch_tiled<DT, 64, true, PARTS, QF>(a, wgs, stream);
   else if (fine)
-    launch_tiled<DT, 128, true, PARTS>(a, wgs, stream);
+    launch_tiled<DT, 128, true, PARTS, QF>(a, wgs, stream);
   else
-    launch_tiled<DT, 128, false, PARTS>(a, wgs, stream);
+    launch_tiled<DT, 128, false, PARTS, QF>(a, wgs, stream);
 }
 
 }  // namespace

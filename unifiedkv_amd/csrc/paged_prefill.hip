@@ -487,31 +487,7 @@ int prefill_impl(const void* q, const void* k_cache, const void* v_cache, const 
   }
   if (fast) {
     const bool fine = fine_shape(head_dim, n_rep);
-    const int64_t pairs = (int64_t)n_groups * batch, rows = (int64_t)total_q * num_q_heads;
-    BlockPlan plan = plan_for(batch, rows, max_chunk, n_groups, head_dim, n_rep, max_blocks, workspace != nullptr);
-    // (the caller sizes the workspace by the same plan; a smaller one runs without parts)
-    if (plan.parts > 1 && (part_bytes(plan.parts, rows, head_dim) > workspace_bytes ||
-                           (rows + 7) / 8 > INT32_MAX || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
-      plan = plan_for(batch, rows, max_chunk, n_groups, head_dim, n_rep, max_blocks, false);
-    a.n3 = plan.n3;
-    a.n2 = plan.n2;
-    a.n_parts = plan.parts;
-    a.part_tiles = plan.part_tiles;
-    a.whole3 = plan.whole3;
-    a.whole2 = plan.whole2;
-    // No more keys than twice the chunk's: the blocks' key counts differ by a factor of two or more, and
-    // every pair's longest blocks go first. (With a long prefix they are alike, and the blocks of one
-    // pair stay together for their XCD's L2.)
-    a.by_block = (int64_t)max_blocks * 16 <= 2 * (int64_t)max_chunk;
-    a.total_q = total_q;
-    if (plan.parts > 1) {
-      a.part_o = static_cast<float*>(workspace);
-      a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + part_o_bytes(plan.parts, rows, head_dim));
-    }
-    // Parts: eight times what an XCD runs at most. (Two parts' items hold a pair's whole blocks: narrow ones are
-    // at least half as wide as wide ones.)
-    const int64_t items = pairs * (a.n3 + a.n2);
-    const int64_t wgs = plan.parts > 1 ? 8 * ((items * plan.parts + 7) / 8) : items;
+    const int64_t wgs = plan_launch(a, total_q, workspace, workspace_bytes);
     // The 64-dim instances write no statistics: every row is flagged, and the scoring pass recomputes
     // them from the keys.
     const int obs_rows = obs && head_dim == 64 ? a.obs : 0;

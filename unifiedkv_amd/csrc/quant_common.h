@@ -27,6 +27,7 @@ struct QuantLayer {
 };
 
 constexpr int kQuantBlock = 32;  // dims that share an exponent
+constexpr int kCache16 = -1;     // in place of a format: pages of the model's type
 
 template <int QF> struct QuantFmt;
 
@@ -95,18 +96,61 @@ template <int QF> __device__ __forceinline__ u32x2 quant_f16x4(uint32_t w, float
   }
 }
 
-// Four codes as two packed pairs of values of the model's type (exact in either).
+// Four codes as two packed pairs of values of a 16-bit type (exact in either). int8 to bf16, whose eight significant
+// bits leave no room for the offset above: through fp32, code + 128 from its byte, times scale, less 128 * scale.
 template <int QF, int DT> __device__ __forceinline__ u32x2 quant_elems4(uint32_t w, float scale) {
-  const u32x2 h = quant_f16x4<QF>(w, scale);
-  if constexpr (DT == UKV_DTYPE_F16) return h;
-  typedef Elem<UKV_DTYPE_F16> E;
-  return u32x2{pack_bf16(E::lo(h[0]), E::hi(h[0])), pack_bf16(E::lo(h[1]), E::hi(h[1]))};
+  if constexpr (DT == UKV_DTYPE_F16) {
+    return quant_f16x4<QF>(w, scale);
+  } else if constexpr (QF == UKV_CACHE_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    const float off = -128.f * scale;
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf((float)(uint8_t)(u >> (8 * i)), scale, off);
+    return u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+  } else {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
+  }
 }
 
 // One code as a float.
 template <int QF> __device__ __forceinline__ float quant_one(uint8_t c, float scale) {
   if constexpr (QF == UKV_CACHE_INT8) return (float)(int8_t)c * scale;
   return __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * scale;
+}
+
+// bf16 queries as fp16 operands: every row is moved by a power of two that its scores' scale takes back. A row whose
+// largest magnitude has the exponent field `top` lands in [2^13, 2^14) with query_to_f16(.., top); 28 binades below
+// that are exact, smaller elements are off by 2^-39 of the largest at most.
+//
+// The largest exponent field of a row, in each of its four lanes (lanes i16 + 16 kg hold eight dims of each step).
+template <int STEPS> __device__ __forceinline__ int query_top(const u32x4 (&q)[STEPS]) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = q[s][c];
+      m = __builtin_elementwise_max(m, as_u16x2(w & 0x7fff7fffu));
+    }
+  int top = max((int)m[0], (int)m[1]) >> 7;
+  top = max(top, __shfl_xor(top, 16));
+  return max(top, __shfl_xor(top, 32));
+}
+template <int STEPS> __device__ __forceinline__ void query_to_f16(u32x4 (&q)[STEPS], int top) {
+  const float down = __uint_as_float((uint32_t)min(267 - top, 254) << 23);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = q[s][c];
+      q[s][c] = pack_f16(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+    }
+}
+// What query_to_f16 divided by.
+__device__ __forceinline__ float query_scale(int top) {
+  return top > 13 ? __uint_as_float((uint32_t)(top - 13) << 23) : 0x1p-127f;
 }
 
 }  // namespace ukv

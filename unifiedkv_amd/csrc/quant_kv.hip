@@ -430,7 +430,5 @@ extern "C" int ukv_quant_prefill(const void* q, const void* k, const void* v, co
   if (rc != UKV_OK) return rc;
   // The chunks hold total_q queries, so the longest holds at least total_q / batch of them.
   if ((int64_t)max_chunk * batch < total_q) return UKV_ERR_INVALID_ARGUMENT;
-  (void)workspace;
-  (void)workspace_bytes;
-  return quant_rows_attention(a, total_q, dtype, format, reinterpret_cast<hipStream_t>(stream));
+  return quant_prefill(a, total_q, dtype, format, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }

@@ -22,6 +22,10 @@ struct QuantAttnArgs {
 int quant_decode(const QuantAttnArgs& a, int dtype, int format, void* workspace, size_t workspace_bytes,
                  hipStream_t stream);
 
+// quant_prefill.hip; the workspace (null: none) is ukv_paged_prefill_workspace_bytes().
+int quant_prefill(const QuantAttnArgs& a, int total_q, int dtype, int format, void* workspace, size_t workspace_bytes,
+                  hipStream_t stream);
+
 int quant_rows_attention(const QuantAttnArgs& a, int rows, int dtype, int format, hipStream_t stream);
 
 }  // namespace ukv
