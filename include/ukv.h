@@ -502,9 +502,12 @@ int ukv_quant_decode(const void* q, const void* k, const void* v, const void* k_
 
 /*
  * ukv_paged_prefill_parts over the 8-bit cache, without statistics: packed chunk queries, causal, bottom right
- * aligned. Workspace as there (ukv_paged_prefill_workspace_bytes; without it the keys stay in one part).
+ * aligned. The workspace (ukv_quant_prefill_workspace_bytes; may be NULL) lets a launch of few queries share its keys
+ * among workgroups; without it each query block takes its keys alone, which a few queries behind long prefixes feel.
  * Replaces core/engine.py:1826-1854 for this cache.
  */
+size_t ukv_quant_prefill_workspace_bytes(int batch, int total_q, int max_chunk, int num_q_heads, int num_kv_heads,
+                                         int head_dim, int n_rep, int max_blocks);
 int ukv_quant_prefill(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale,
                       const int64_t* layer_strides, int num_pages, const int32_t* block_table,
                       const int32_t* cu_seqlens_q, const int32_t* kv_lens, void* out, int batch, int total_q,

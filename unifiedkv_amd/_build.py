@@ -30,6 +30,7 @@ SOURCES = [
     "paged_prefill.hip",
     "snapkv_score.hip",
     "quant_kv.hip",
+    "quant_split.hip",
     "quant_prefill.hip",
 ]
 

@@ -247,6 +247,8 @@ SIGNATURES = {
             ctypes.c_float, _c_int, _c_int, _c_void_p, ctypes.c_size_t, _c_void_p,  # scale format dtype ws bytes stream
         ],
     ),
+    "ukv_quant_prefill_workspace_bytes": (
+        ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "ukv_quant_prefill": (
         _c_int,
         [

@@ -29,143 +29,12 @@
 // A reference-faithful scalar kernel (natural exp, one workgroup per (b, h))
 // serves shapes the split kernel is not instantiated for (head_dim not in
 // {64, 128, 256}, n_rep > 16, or rows not 16-byte aligned).
-#include <algorithm>
-#include <atomic>
-#include <cmath>
-#include <cstdlib>
-#include <cstring>
-#include <type_traits>
-
-#include "quant_common.h"
-#include "quant_rows.h"
+#include "page16_split.h"
 
 namespace ukv {
 
-struct DecodeArgs {
-  const uint16_t* q;
-  const uint16_t* k;
-  const uint16_t* v;
-  const int32_t* bt;
-  const int32_t* lens;
-  uint16_t* out;
-  float* part_o;     // [slots][Hq][D], slots = grid_wgs + B
-  float2* part_ml;   // [slots][Hq]: (running max in log2 units, sum of exp2)
-  int32_t* seq_start;  // [B] first global page of each sequence (written by workgroup 0); entry 0, whose
-                       // page is 0, holds the shares the pages were cut into
-  int32_t* seq_pages;  // [B] pages of each sequence
-  int64_t q_sb, q_sh;
-  int64_t k_sp, k_st, k_sh;
-  int64_t v_sp, v_st, v_sh;
-  int B, Hq, n_rep, n_groups, D, max_blocks, num_pages;
-  int grid_wgs;      // workgroups sharing the batch's pages (the most shares they are cut into)
-  int fixed_shares;  // cut them into exactly grid_wgs shares (launch-shape sweeps)
-  int subs;          // waves of a workgroup that share each KV head's pages (split kernel, SHARED)
-  // Decode-token append (fused variant): k_new/v_new [B][n_groups][D] rows with
-  // strides n_sb, n_sh; the token of sequence b goes to position lens[b] - 1.
-  const uint16_t* k_new;
-  const uint16_t* v_new;
-  int64_t n_sb, n_sh;
-  float scale;       // natural-log units (scalar kernel)
-  float scale_log2;  // scale * log2(e) (split kernel)
-};
-
-// The 8-bit cache (QF: its format; kCache16: pages of the model's type): k and v are bytes, with strides in
-// bytes, and these their exponents.
-struct QuantDecodeArgs : DecodeArgs {
-  const uint8_t* ks;
-  const uint8_t* vs;
-  int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
-};
-template <int QF> struct SplitArgs { typedef QuantDecodeArgs type; };
-template <> struct SplitArgs<kCache16> { typedef DecodeArgs type; };
-
-__device__ __forceinline__ int clamp_len(int L, int max_blocks) {
-  const int cap = max_blocks * 16;
-  return L < 0 ? 0 : (L > cap ? cap : L);
-}
-
-__device__ __forceinline__ int pages_of(int len, int max_blocks) { return (clamp_len(len, max_blocks) + 15) >> 4; }
-
-// floor(x * y / z) for 0 <= x, y and 0 < z: one 32-bit division where the product fits.
-__device__ __forceinline__ int mul_div(int x, int y, int z) {
-  const uint64_t p = (uint64_t)(uint32_t)x * (uint32_t)y;
-  if ((p >> 32) == 0) return (int)((uint32_t)p / (uint32_t)z);
-  return (int)(p / (uint32_t)z);
-}
-
-// Largest of the wave's 64 values (>= 0), in every lane.
-__device__ __forceinline__ int wave_max_i32(int x) {
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
-  return __builtin_amdgcn_readlane(x, 63);
-}
-
-// Shares the batch's P pages are cut into, at most G. The host sees the table's width alone; here the
-// lengths say how much there is to share: a page more in a share costs ~0.85 us, a share more of the
-// longest sequence ~0.05 us in the merge, so a share takes about sqrt(longest) / 4 pages. One sequence
-// of 4096 tokens beside three of 17: 16.8 us with 72 shares, 23.9 with 256, 21.2 with 32; four of 128
-// pages keep their 128 shares. A multiple of 8 (G too, or it is taken whole) for the XCDs' equal runs.
-// With P >= G^2 / 16 + 2 G the rule gives G whatever the longest (a share takes at most
-// sqrt(P) / 4 + 1/2 pages), and neither it nor the square root is waited for.
-template <class F>
-__device__ __forceinline__ int shares_for(const DecodeArgs& a, int P, F longest_pages) {
-  const int many = (int)min((int64_t)INT32_MAX, (int64_t)a.grid_wgs * (a.grid_wgs + 32) / 16 + 1);
-  if (a.fixed_shares || P >= many) return a.grid_wgs;
-  const int longest = longest_pages();
-  // (the square root is vector code: its result back to a scalar register, with all that follows from it; three
-  // more vector registers would leave the 64-dim split one workgroup to a CU)
-  const int per = max(1, __builtin_amdgcn_readfirstlane((int)(0.25f * __builtin_sqrtf((float)longest) + 0.5f)));
-  return min(a.grid_wgs, max(8, ((P + per - 1) / per + 7) & ~7));
-}
-
-// Splits fp32 softmax weights into two 16-bit parts (p ~= hi + lo, relative
-// error below 2^-16) so that P.V can run on 16-bit MFMA with fp32-grade
-// weights. The fp16 path scales p by 2^7 first so small weights stay normal.
-template <int DT> struct PSplit;
-
-template <> struct PSplit<UKV_DTYPE_BF16> {
-  static constexpr float kScale = 1.f;
-  static __device__ __forceinline__ uint32_t pack(float x0, float x1) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, bf16x2));
-  }
-  static __device__ __forceinline__ void split(const float (&p)[4], u32x2& hi, u32x2& lo) {
-    hi = u32x2{pack(p[0], p[1]), pack(p[2], p[3])};
-    const float r0 = p[0] - __uint_as_float(hi[0] << 16), r1 = p[1] - __uint_as_float(hi[0] & 0xffff0000u);
-    const float r2 = p[2] - __uint_as_float(hi[1] << 16), r3 = p[3] - __uint_as_float(hi[1] & 0xffff0000u);
-    lo = u32x2{pack(r0, r1), pack(r2, r3)};
-  }
-};
-
-template <> struct PSplit<UKV_DTYPE_F16> {
-  static constexpr float kScale = 128.f;
-  static __device__ __forceinline__ uint32_t pack(float x0, float x1) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-  }
-  static __device__ __forceinline__ void split(const float (&pin)[4], u32x2& hi, u32x2& lo) {
-    float p[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) p[r] = pin[r] * kScale;
-    hi = u32x2{pack(p[0], p[1]), pack(p[2], p[3])};
-    const float r0 = p[0] - Elem<UKV_DTYPE_F16>::lo(hi[0]), r1 = p[1] - Elem<UKV_DTYPE_F16>::hi(hi[0]);
-    const float r2 = p[2] - Elem<UKV_DTYPE_F16>::lo(hi[1]), r3 = p[3] - Elem<UKV_DTYPE_F16>::hi(hi[1]);
-    lo = u32x2{pack(r0, r1), pack(r2, r3)};
-  }
-};
-
 #ifndef UKV_PAGE16_NT
 #define UKV_PAGE16_NT 1
-#endif
-#ifndef UKV_PAGE16_WAVES
-#define UKV_PAGE16_WAVES 8
-#endif
-#ifndef UKV_QUANT_PIPE
-#define UKV_QUANT_PIPE 3
 #endif
 #ifndef UKV_PAGE16_MIN_WAVES_PER_EU
 #define UKV_PAGE16_MIN_WAVES_PER_EU 1
@@ -214,41 +83,6 @@ __device__ __forceinline__ void load_vrow(const uint16_t* p, VRow<DPL>& r) {
   }
 }
 
-// One lane's part of a page as loaded: dims DPL * i16 .. of tokens 4 * kg + t, and, of the 8-bit cache, those
-// tokens' exponents of the block the dims lie in (token t's in byte t).
-template <int DPL, int QF> struct PageRows {
-  struct Row { uint32_t w[DPL / 4]; };
-  Row k[4], v[4];
-  uint32_t ke, ve;
-};
-template <int DPL> struct PageRows<DPL, kCache16> { VRow<DPL> k[4], v[4]; };
-
-template <int DPL, class R> __device__ __forceinline__ void load_codes(const uint8_t* p, R& r) {
-  if constexpr (DPL == 4) {
-    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
-  } else if constexpr (DPL == 8) {
-    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
-    r.w[0] = x[0];
-    r.w[1] = x[1];
-  } else {
-    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-#pragma unroll
-    for (int c = 0; c < 4; ++c) r.w[c] = x[c];
-  }
-}
-
-// Codes -> fp16 values. An exponent byte of 255 is 2^128, infinity: zero codes make NaN of it, e4m3's are NaN.
-template <int DPL, int QF, class R>
-__device__ __forceinline__ void widen(const R& r, uint32_t exps, int t, VRow<DPL>& out) {
-  const float scale = __uint_as_float((exps >> (8 * t) & 255u) << 23);
-#pragma unroll
-  for (int c = 0; c < DPL / 4; ++c) {
-    const u32x2 x = quant_f16x4<QF>(r.w[c], scale);
-    out.w[2 * c] = x[0];
-    out.w[2 * c + 1] = x[1];
-  }
-}
-
 // Split-K Page16 decode, one wave per KV head, all of that head's q heads
 // (up to 16) per KV read.
 //
@@ -286,23 +120,12 @@ __device__ __forceinline__ void widen(const R& r, uint32_t exps, int t, VRow<DPL
 // DIRECT (short tables): workgroup (b, g) takes the whole of sequence b for KV head g, its waves
 // sharing the pages as under SHARED, and writes the output itself: no partials, no second kernel, and
 // the table row is read beside the length instead of after it.
-//
-// QF: K and V are 8-bit codes (quant_common.h). A page's codes stay in the registers as loaded until the page is
-// reduced, then become fp16 values, which they are exactly, and go the way of an fp16 page; bf16 queries become fp16
-// too, moved by a power of two for each row that the scale takes back (28 binades below a row's largest value are
-// exact). Half the bytes a page: twice the pages in flight for the same cover of HBM's latency.
-enum SplitMode { kSplit = 0, kShared = 1, kDirect = 2 };
-template <int DT, int D, bool APPEND, int MODE, int QF = kCache16>
-__global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PER_EU)
-page16_split_kernel(const typename SplitArgs<QF>::type a) {
-  constexpr bool QUANT = QF != kCache16;
-  constexpr int MT = QUANT ? (int)UKV_DTYPE_F16 : DT;  // the type the matrix cores take
-  static_assert(!(QUANT && APPEND), "the 8-bit append is a kernel of its own");
+template <int DT, int D, bool APPEND, int MODE>
+__global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, UKV_PAGE16_MIN_WAVES_PER_EU) page16_split_kernel(const DecodeArgs a) {
   constexpr int STEPS = D / 32;  // QK k-steps of 32 dims
   constexpr int DPL = D / 16;    // V dims per lane = P.V output tiles
   constexpr float kTau = 8.f;
-  // register sets (D=256 has no registers for a second page)
-  constexpr int kPipe = D > 128 ? 1 : QUANT ? UKV_QUANT_PIPE : 2;
+  constexpr int kPipe = D > 128 ? 1 : 2;  // register sets (D=256 has no registers for a second page)
 
   const int lane = threadIdx.x & 63;
   const int wv = threadIdx.x >> 6;
@@ -398,8 +221,7 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
   const int n_here = min(a.n_rep, a.Hq - qh0);
   const bool live = i16 < n_here;
 
-  typedef std::conditional_t<QUANT, uint8_t, uint16_t> CacheElem;
-  const CacheElem* kbase = (const CacheElem*)a.k + (int64_t)(4 * kg) * a.k_st + (int64_t)g * a.k_sh + DPL * i16;
+  const uint16_t* kbase = a.k + (int64_t)(4 * kg) * a.k_st + (int64_t)g * a.k_sh + DPL * i16;
   // Wave-private LDS rows of the page's K (token-major): rows are loaded 4 tokens
   // x full width per instruction and read back in MFMA layout. The pitch of D + 16
   // elements (288 B at D = 128) keeps SQ_LDS_BANK_CONFLICT at 0 for the 16-row
@@ -410,7 +232,7 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
   // SHARED: the waves' partial rows and (m, l) of a segment.
   __shared__ __attribute__((aligned(16))) float part_lds[SHARED ? UKV_PAGE16_WAVES * 16 * D : 4];
   __shared__ float2 ml_lds[SHARED ? UKV_PAGE16_WAVES * 16 : 1];
-  const CacheElem* vbase = (const CacheElem*)a.v + (int64_t)(4 * kg) * a.v_st + (int64_t)g * a.v_sh + DPL * i16;
+  const uint16_t* vbase = a.v + (int64_t)(4 * kg) * a.v_st + (int64_t)g * a.v_sh + DPL * i16;
 
   // Per-segment state (one sequence's share of this workgroup's pages).
   int b = b_first;   // current sequence
@@ -427,7 +249,6 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
   VRow<DPL> vtok;      // APPEND: the new V row (lanes kg == tail_slot / 4)
 
   u32x4 qb[STEPS];   // B operand of QK^T: column i16 = q head qh0 + i16 (zero beyond n_here)
-  float q_scale = 0.f;  // QUANT: the scale of head i16's scores (log2 units), its row's power of two included
   float m_ref;       // running max of head i16 (log2 units)
   float lsum;        // this lane's share of that head's sum of weights
   f32x4 acc[DPL];
@@ -435,8 +256,7 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
   auto page_window = [&](int i0) {
     bid_win = i0 + lane < n_mine ? btrow[SHARED ? pa + sub + (i0 + lane) * subs : pa + i0 + lane] : 0;
   };
-  typedef PageRows<DPL, QF> Page;
-  auto load_page = [&](int idx, Page& pg, int& nv) {
+  auto load_page = [&](int idx, VRow<DPL> (&kr)[4], VRow<DPL> (&vr)[4], int& nv) {
     const int p = SHARED ? pa + sub + idx * subs : pa + idx;
     if (!DIRECT && idx != 0 && (idx & 63) == 0) page_window(idx);
     int bid = __builtin_amdgcn_readlane(bid_win, idx & 63);
@@ -445,22 +265,12 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
       if (p == tail_page) tail_pid = ok ? bid : -1;
     bid = ok ? bid : 0;
     nv = ok ? min(16, L - 16 * p) : 0;
-    const CacheElem* kp = kbase + (int64_t)bid * a.k_sp;
-    const CacheElem* vp = vbase + (int64_t)bid * a.v_sp;
-    if constexpr (QUANT) {
-      const int64_t h = g, blk = DPL * i16 / kQuantBlock;
+    const uint16_t* kp = kbase + (int64_t)bid * a.k_sp;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) load_codes<DPL>(kp + (int64_t)t * a.k_st, pg.k[t]);
-      pg.ke = *reinterpret_cast<const uint32_t*>(a.ks + bid * a.ks_sp + h * a.ks_sh + blk * a.ks_sb + 4 * kg);
+    for (int t = 0; t < 4; ++t) load_vrow<DPL>(kp + (int64_t)t * a.k_st, kr[t]);
+    const uint16_t* vp = vbase + (int64_t)bid * a.v_sp;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) load_codes<DPL>(vp + (int64_t)t * a.v_st, pg.v[t]);
-      pg.ve = *reinterpret_cast<const uint32_t*>(a.vs + bid * a.vs_sp + h * a.vs_sh + blk * a.vs_sb + 4 * kg);
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) load_vrow<DPL>(kp + (int64_t)t * a.k_st, pg.k[t]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) load_vrow<DPL>(vp + (int64_t)t * a.v_st, pg.v[t]);
-    }
+    for (int t = 0; t < 4; ++t) load_vrow<DPL>(vp + (int64_t)t * a.v_st, vr[t]);
   };
 
   // APPEND: on the token's page, its slot gets the new rows (per-lane register selects).
@@ -484,10 +294,10 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
     for (int s = 0; s < STEPS; ++s) ka[s] = *reinterpret_cast<const u32x4*>(ks + i16 * KP + 8 * kg + 32 * s);
     f32x4 sacc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) sacc = mfma16x16x32<MT>(ka[s], qb[s], sacc);
+    for (int s = 0; s < STEPS; ++s) sacc = mfma16x16x32<DT>(ka[s], qb[s], sacc);
     float s2[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s2[r] = sacc[r] * (QUANT ? q_scale : a.scale_log2);
+    for (int r = 0; r < 4; ++r) s2[r] = sacc[r] * a.scale_log2;
     if (nv < 16) {  // last page of the sequence or an invalid page id
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -520,22 +330,23 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
       lsum += p[r];
     }
     u32x2 phi, plo;
-    PSplit<MT>::split(p, phi, plo);
+    PSplit<DT>::split(p, phi, plo);
 #pragma unroll
     for (int c = 0; c < DPL / 2; ++c) {
       const u32x2 blo = {__builtin_amdgcn_perm(vr[1].w[c], vr[0].w[c], 0x05040100u),
                          __builtin_amdgcn_perm(vr[3].w[c], vr[2].w[c], 0x05040100u)};
       const u32x2 bhi = {__builtin_amdgcn_perm(vr[1].w[c], vr[0].w[c], 0x07060302u),
                          __builtin_amdgcn_perm(vr[3].w[c], vr[2].w[c], 0x07060302u)};
-      acc[2 * c] = mfma16x16x16<MT>(phi, blo, acc[2 * c]);
-      acc[2 * c] = mfma16x16x16<MT>(plo, blo, acc[2 * c]);
-      acc[2 * c + 1] = mfma16x16x16<MT>(phi, bhi, acc[2 * c + 1]);
-      acc[2 * c + 1] = mfma16x16x16<MT>(plo, bhi, acc[2 * c + 1]);
+      acc[2 * c] = mfma16x16x16<DT>(phi, blo, acc[2 * c]);
+      acc[2 * c] = mfma16x16x16<DT>(plo, blo, acc[2 * c]);
+      acc[2 * c + 1] = mfma16x16x16<DT>(phi, bhi, acc[2 * c + 1]);
+      acc[2 * c + 1] = mfma16x16x16<DT>(plo, bhi, acc[2 * c + 1]);
     }
   };
 
-  constexpr float kUnscale = 1.f / PSplit<MT>::kScale;
-  Page pages[kPipe];
+  constexpr float kUnscale = 1.f / PSplit<DT>::kScale;
+  VRow<DPL> kb[kPipe][4];
+  VRow<DPL> vb[kPipe][4];
   int nvb[kPipe];
   int seg_start = s_first;  // global index of page 0 of sequence b
   int x = x0;
@@ -568,33 +379,16 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
       const uint16_t* qp = a.q + (int64_t)b * a.q_sb + (int64_t)(qh0 + (live ? i16 : 0)) * a.q_sh + 8 * kg;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) qb[s] = live ? ld16(qp + 32 * s) : u32x4{0u, 0u, 0u, 0u};
-      if constexpr (QUANT) {
-        q_scale = a.scale_log2;
-        if constexpr (DT == UKV_DTYPE_BF16) {
-          const int top = query_top<STEPS>(qb);
-          query_to_f16<STEPS>(qb, top);
-          q_scale *= query_scale(top);
-        }
-      }
     }
     m_ref = kNegFltMax;
     lsum = 0.f;
 #pragma unroll
     for (int e = 0; e < DPL; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto reduce = [&](int i, Page& pg, int nv) {
+    auto reduce = [&](int i, VRow<DPL> (&kr)[4], VRow<DPL> (&vr)[4], int nv) {
       if constexpr (APPEND)
-        if ((SHARED ? pa + sub + i * subs : pa + i) == tail_page) swap_in_token(pg.k, pg.v);
-      if constexpr (QUANT) {
-        VRow<DPL> kr[4], vr[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) widen<DPL, QF>(pg.k[t], pg.ke, t, kr[t]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) widen<DPL, QF>(pg.v[t], pg.ve, t, vr[t]);
-        process_page(kr, vr, nv);
-      } else {
-        process_page(pg.k, pg.v, nv);
-      }
+        if ((SHARED ? pa + sub + i * subs : pa + i) == tail_page) swap_in_token(kr, vr);
+      process_page(kr, vr, nv);
     };
     if constexpr (DIRECT) {
       // Page i + 1 is in flight while page i is reduced: every load of the loop is unconditional, so
@@ -603,35 +397,35 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
       // saturate HBM, are 2 % faster with that one).
       constexpr int B1 = kPipe - 1;
       if (n_mine > 0) {
-        load_page(0, pages[0], nvb[0]);
+        load_page(0, kb[0], vb[0], nvb[0]);
         int i = 0;
         for (; i + 2 < n_mine; i += 2) {
-          load_page(i + 1, pages[B1], nvb[B1]);
-          reduce(i, pages[0], nvb[0]);
-          load_page(i + 2, pages[0], nvb[0]);
-          reduce(i + 1, pages[B1], nvb[B1]);
+          load_page(i + 1, kb[B1], vb[B1], nvb[B1]);
+          reduce(i, kb[0], vb[0], nvb[0]);
+          load_page(i + 2, kb[0], vb[0], nvb[0]);
+          reduce(i + 1, kb[B1], vb[B1], nvb[B1]);
         }
         if (i + 1 < n_mine) {
-          load_page(i + 1, pages[B1], nvb[B1]);
-          reduce(i, pages[0], nvb[0]);
-          reduce(i + 1, pages[B1], nvb[B1]);
+          load_page(i + 1, kb[B1], vb[B1], nvb[B1]);
+          reduce(i, kb[0], vb[0], nvb[0]);
+          reduce(i + 1, kb[B1], vb[B1], nvb[B1]);
         } else {
-          reduce(i, pages[0], nvb[0]);
+          reduce(i, kb[0], vb[0], nvb[0]);
         }
       }
     } else {
       // Register sets in turn: the loads of page i + kPipe - 1 are issued before page i is reduced.
 #pragma unroll
       for (int i = 0; i < kPipe - 1; ++i)
-        if (i < n_mine) load_page(i, pages[i], nvb[i]);
+        if (i < n_mine) load_page(i, kb[i], vb[i], nvb[i]);
       for (int base = 0; base < n_mine; base += kPipe) {
 #pragma unroll
         for (int u = 0; u < kPipe; ++u) {
           const int i = base + u;
           if (i < n_mine) {
             const int nxt = (u + kPipe - 1) % kPipe;  // constant after unrolling
-            if (i + kPipe - 1 < n_mine) load_page(i + kPipe - 1, pages[nxt], nvb[nxt]);
-            reduce(i, pages[u], nvb[u]);
+            if (i + kPipe - 1 < n_mine) load_page(i + kPipe - 1, kb[nxt], vb[nxt], nvb[nxt]);
+            reduce(i, kb[u], vb[u], nvb[u]);
           }
         }
       }
@@ -712,121 +506,6 @@ page16_split_kernel(const typename SplitArgs<QF>::type a) {
   }
 }
 
-// Maximum / sum over the wave's 64 lanes, in every lane (the steps of wave_inclusive_scan_i32).
-#define UKV_WAVE_REDUCE(x, op, old)                                                                        \
-  x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(old, __float_as_int(x), 0x111, 0xf, 0xf, false))); \
-  x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(old, __float_as_int(x), 0x112, 0xf, 0xf, false))); \
-  x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(old, __float_as_int(x), 0x114, 0xf, 0xf, false))); \
-  x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(old, __float_as_int(x), 0x118, 0xf, 0xf, false))); \
-  x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(old, __float_as_int(x), 0x142, 0xa, 0xf, false))); \
-  x = op(x, __int_as_float(__builtin_amdgcn_update_dpp(old, __float_as_int(x), 0x143, 0xc, 0xf, false)));
-__device__ __forceinline__ float wave_max(float x) {
-  UKV_WAVE_REDUCE(x, fmaxf, (int)0xff800000)  // -inf
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
-}
-__device__ __forceinline__ float add_f32(float x, float y) { return x + y; }
-__device__ __forceinline__ float wave_sum(float x) {
-  UKV_WAVE_REDUCE(x, add_f32, 0)
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
-}
-
-// Merges the partials of one (sequence, q head): log-sum-exp in log2 units.
-// The sequence's pages [S, S+n) of the batch's P pages were split over
-// shares w = floor(((S+1)G - 1)/P) .. floor(((S+n)G - 1)/P), whose partials
-// sit in slots w + b. 256 threads: thread (cs, dq) owns float4 dims 4*dq.. of
-// partials cs, cs+CS, ...; it issues the loads of its first kPre rows together
-// with the (m, l) loads, so that one memory round trip serves both. Every wave computes
-// all the weights itself, with register reductions, and reads back what it wrote to LDS
-// (every wave writes the same values): the one barrier is the CS partial sums' meeting in LDS.
-template <int DT, int D>
-__global__ void __launch_bounds__(256) page16_combine_kernel(const DecodeArgs a) {
-  constexpr int TD = D / 4;       // threads per partial row (float4 each)
-  constexpr int CS = 256 / TD;    // chunk groups
-  constexpr int kPre = 4;         // partial rows per thread loaded before the weights
-  extern __shared__ float sums[];  // [CS][D] sums, then [grid_wgs] weights
-
-  const int h = blockIdx.x;
-  const int b = blockIdx.y;
-  const int tid = threadIdx.x;
-  const int n_pages = a.seq_pages[b];
-  const int P = (a.B > 1 ? a.seq_start[a.B - 1] : 0) + a.seq_pages[a.B - 1];
-  const int S = b > 0 ? a.seq_start[b] : 0;
-  const int G = a.seq_start[0];
-  auto share_of = [&](int x) -> int {  // floor(((x + 1) G - 1) / P): the share holding page x
-    const uint64_t p = (uint64_t)(uint32_t)(x + 1) * (uint32_t)G - 1;
-    return (p >> 32) == 0 ? (int)((uint32_t)p / (uint32_t)P) : (int)(p / (uint32_t)P);
-  };
-  const int w_first = n_pages > 0 ? share_of(S) : 0;
-  const int w_last = n_pages > 0 ? share_of(S + n_pages - 1) : -1;
-  const int n_chunks = w_last - w_first + 1;
-  const int64_t base = (int64_t)(w_first + b) * a.Hq + h;
-  // With fewer pages than workgroups (P < G) some workgroups in [w_first, w_last]
-  // own no page and wrote no partial: their slots hold stale data and are skipped.
-  auto owns_pages = [&](int c) {
-    const int w = w_first + c;
-    return P >= G || mul_div(w + 1, P, G) > mul_div(w, P, G);
-  };
-
-  const int cs = tid / TD;
-  const int dq = tid % TD;
-  const float* po = a.part_o + base * D + 4 * dq;
-  const int64_t cstride = (int64_t)a.Hq * D;
-  f32x4 rows[kPre];  // partials cs + k*CS (in the workspace even when stale; skipped below)
-#pragma unroll
-  for (int k = 0; k < kPre; ++k) {
-    const int c = cs + k * CS;
-    rows[k] = c < n_chunks ? *reinterpret_cast<const f32x4*>(po + (int64_t)c * cstride) : f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const int lane = tid & 63;
-  float* w_s = sums + CS * D;
-  const bool own0 = lane < n_chunks && owns_pages(lane);
-  const float2 ml0 = own0 ? a.part_ml[base + (int64_t)lane * a.Hq] : make_float2(-INFINITY, 0.f);
-
-  float mx = ml0.x;
-  for (int c = lane + 64; c < n_chunks; c += 64)
-    if (owns_pages(c)) mx = fmaxf(mx, a.part_ml[base + (int64_t)c * a.Hq].x);
-  const float M = wave_max(mx);
-  float dsum = 0.f;
-  for (int c = lane; c < n_chunks; c += 64) {
-    const bool own = c == lane ? own0 : owns_pages(c);
-    if (!own) {
-      w_s[c] = -1.f;  // marks an empty slot (real weights are >= 0 or NaN)
-      continue;
-    }
-    const float2 ml = c == lane ? ml0 : a.part_ml[base + (int64_t)c * a.Hq];
-    const float w = exp2f(ml.x - M);
-    w_s[c] = w;
-    dsum += ml.y * w;
-  }
-  const float den = wave_sum(dsum);
-  // the wave's own LDS writes, by other lanes, before the reads below
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < kPre; ++k) {
-    const int c = cs + k * CS;
-    if (c < n_chunks) {
-      const float w = w_s[c];
-      if (!(w < 0.f)) acc += w * rows[k];
-    }
-  }
-#pragma unroll 4
-  for (int c = cs + kPre * CS; c < n_chunks; c += CS) {
-    const float w = w_s[c];
-    if (!(w < 0.f)) acc += w * *reinterpret_cast<const f32x4*>(po + (int64_t)c * cstride);
-  }
-  *reinterpret_cast<f32x4*>(sums + cs * D + 4 * dq) = acc;
-  __syncthreads();
-  if (tid < D) {
-    float num = 0.f;
-#pragma unroll
-    for (int g = 0; g < CS; ++g) num += sums[g * D + tid];
-    a.out[((int64_t)b * a.Hq + h) * D + tid] = Elem<DT>::from_float(n_chunks > 0 ? num / den : NAN);
-  }
-}
-
 // One workgroup per (q head, sequence); the same arithmetic as the reference
 // Triton program: natural exp, -FLT_MAX for masked scores, page loop in order.
 template <int DT>
@@ -885,180 +564,44 @@ __global__ void __launch_bounds__(256) page16_scalar_kernel(const DecodeArgs a) 
 // ---------------------------------------------------------------------------
 namespace {
 
-constexpr int kMinPagesPerWg = 4;  // below this a workgroup's setup outweighs its pages
-
-// CU count of the current device, cached per device id (0 = not yet read; a
-// racing first read stores the same value twice).
-int device_cu_count() {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
-  if (dev < 64) {
-    const int c = cached[dev].load(std::memory_order_relaxed);
-    if (c > 0) return c;
-  }
-  int cus = 0;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
-  if (dev < 64) cached[dev].store(cus, std::memory_order_relaxed);
-  return cus;
-}
-
-// UKV_PAGE16_WGS, read once per process (0 when unset or not a positive number).
-int env_wgs() {
-  static const int v = [] {
-    const char* env = std::getenv("UKV_PAGE16_WGS");
-    const int x = (env && *env) ? std::atoi(env) : 0;
-    return x > 0 ? std::min(x, 65535) : 0;
-  }();
-  return v;
-}
-
-// Workgroups G sharing the batch's pages: one per CU (a single round of equal
-// workgroups measured fastest), fewer when even the largest possible batch
-// (batch * max_blocks pages) gives each fewer than kMinPagesPerWg pages, but one per sequence (a
-// workgroup takes its segments one after another); a multiple of 8 for the XCDs' equal runs. The lengths
-// may lower it on the device (shares_for). Partials
-// beyond kMaxPartials bytes keep the coarser rule. UKV_PAGE16_WGS overrides it for launch-shape sweeps.
-constexpr size_t kMaxPartials = size_t(16) << 20;
-long long coarse_wgs(int batch, int max_blocks) {  // one per eight pages the table holds
-  const long long bound = (long long)batch * (long long)std::max(max_blocks, 1);
-  return std::max<long long>(1, std::min<long long>(device_cu_count(), (bound + 7) / 8));
-}
-long long fine_wgs(int batch, int max_blocks) {
-  const long long bound = (long long)batch * (long long)std::max(max_blocks, 1);
-  const long long want = std::max<long long>((bound + kMinPagesPerWg - 1) / kMinPagesPerWg, batch);
-  return std::max(coarse_wgs(batch, max_blocks), std::min<long long>(device_cu_count(), (want + 7) / 8 * 8));
-}
-int split_wgs_for(int batch, int hq, int d, int max_blocks) {
-  if (const int v = env_wgs()) return v;
-  const long long g = fine_wgs(batch, max_blocks);
-  const bool fits = (size_t)(g + batch) * hq * (d + 2) * sizeof(float) <= kMaxPartials;
-  return (int)(fits ? g : coarse_wgs(batch, max_blocks));
-}
-
-// More KV heads than a workgroup's waves take several workgroups a share: the finer split stops where these
-// fill the CUs, as a second round costs more than it spreads (4 x 4096 tokens on 16 heads of 128 dims, one
-// workgroup to a CU: 26.4 us with 128 shares, 37 with 256).
-int launch_wgs(int wgs, int batch, int max_blocks, int n_groups) {
-  const int per_share = (n_groups + UKV_PAGE16_WAVES - 1) / UKV_PAGE16_WAVES;
-  if (per_share == 1 || env_wgs()) return wgs;
-  const int one_round = std::max(8, (device_cu_count() / per_share) & ~7);
-  return (int)std::max<long long>(coarse_wgs(batch, max_blocks), std::min(wgs, one_round));
-}
-
-// kDirect: a CU streams at most ~47 GB/s (32 KB in flight against ~0.7 us), so a sequence on one
-// workgroup per KV head pays only while its pages are few: per layer of a step at 512 tokens 7-10 us
-// against 9-13 (1-8 sequences) and 14.5 / 24.7 against 19.4 / 29.3 us (32 / 64 sequences, 8 KV heads). At
-// 1024 it wins where the (sequence, head) pairs fill half of the CUs (17 against 21 us at 128 pairs, 24
-// against 29 at 256) and loses below (15.7 against 14.3 us at 8 x 8, 11.4 against 9.4 at 8 x 1). Pairs
-// beyond the workgroups the device holds (one to a CU at 128 dims, two at 64) wait ~2.9 us a round behind
-// the short sequences before a long one starts: 64 sequences on 8 heads, one of 1024 tokens among 17s, took
-// 20.2 us against 15.3 for the split. There the longer tables are left to the split, and with few q heads a KV
-// head, whose merge is cheap, all but the shortest (as many q heads as KV heads, one long sequence: 32 x 16 in
-// 24 pages 12.6 against 11.3 us, 64 x 16 in 16 pages 16.1 against 14.5; 128 x 8 at two q heads a KV head in 32
-// pages 18.4 against 16.1, in 16 pages 15 against 17; 256 x 16 one-page sequences 41 against 35).
-constexpr int kDirectPages = 32, kDirectPagesWide = 64;
-bool direct_shape(int batch, int n_groups, int n_rep, int head_dim, int max_blocks) {
-  if (head_dim > 128 || n_groups > 65535 || env_wgs()) return false;
-  const long long pairs = (long long)batch * n_groups, cus = device_cu_count();
-  const long long held = head_dim == 64 ? 2 * cus : cus;
-  if (max_blocks > (pairs >= cus / 2 && pairs <= cus ? kDirectPagesWide : kDirectPages)) return false;
-  if (pairs <= held || n_rep >= 4 || (head_dim == 64 && n_groups <= UKV_PAGE16_WAVES)) return true;
-  return pairs <= 8 * held && pairs * max_blocks <= held * (head_dim == 64 ? 48 : n_rep == 1 ? 40 : 80);
-}
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-
-struct WorkspaceLayout {
-  size_t part_o_off, part_ml_off, seq_off, total;
-  int wgs;
-};
-
-// [slots][Hq][D] fp32 partials, [slots][Hq] (m, l), then the per-sequence page
-// starts and counts; slots = G + batch.
-WorkspaceLayout layout_of(int wgs, int batch, int hq, int d) {
-  WorkspaceLayout w{};
-  w.wgs = wgs;
-  const size_t slots = ((size_t)w.wgs + (size_t)batch) * hq;
-  w.part_o_off = 0;
-  w.part_ml_off = align256(slots * d * sizeof(float));
-  w.seq_off = w.part_ml_off + align256(slots * sizeof(float2));
-  w.total = w.seq_off + align256(2 * (size_t)batch * sizeof(int32_t));
-  return w;
-}
-WorkspaceLayout workspace_layout(int batch, int hq, int d, int max_blocks) {
-  return layout_of(split_wgs_for(batch, hq, d, max_blocks), batch, hq, d);
-}
-
-// What the size query reports: no less than workspace_layout() takes, and never less for a larger batch,
-// table or head shape, so that one buffer sized for the largest serves the smaller ones (the layout itself
-// shrinks where the partials pass kMaxPartials).
-size_t workspace_report(int batch, int hq, int d, int max_blocks) {
-  if (env_wgs()) return workspace_layout(batch, hq, d, max_blocks).total;
-  const size_t fine = layout_of((int)fine_wgs(batch, max_blocks), batch, hq, d).total;
-  const size_t coarse = layout_of((int)coarse_wgs(batch, max_blocks), batch, hq, d).total;
-  const size_t most_fine = kMaxPartials + 2 * 256 + align256(2 * (size_t)batch * sizeof(int32_t));  // where it fits
-  return std::max(coarse, std::min(fine, most_fine));
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// (the split kernel of a cache and a mode, with and without the append)
-template <int DT, int D, int MODE, int QF>
-void launch_mode(const typename SplitArgs<QF>::type& a, dim3 grid, dim3 block, hipStream_t stream) {
-  if constexpr (QF == kCache16)
-    if (a.k_new) {
-      hipLaunchKernelGGL((page16_split_kernel<DT, D, true, MODE, QF>), grid, block, 0, stream, a);
-      return;
-    }
-  hipLaunchKernelGGL((page16_split_kernel<DT, D, false, MODE, QF>), grid, block, 0, stream, a);
-}
-
-template <int DT, int D, int QF>
-void launch_split(const typename SplitArgs<QF>::type& a, hipStream_t stream) {
+template <int DT, int D>
+void launch_split(const DecodeArgs& a, hipStream_t stream) {
   // Waves left over by the KV heads share the heads' pages (D = 256 has no LDS for their rows).
   if constexpr (D <= 128) {
     if (direct_shape(a.B, a.n_groups, a.n_rep, a.D, a.max_blocks)) {
-      launch_mode<DT, D, kDirect, QF>(a, dim3(a.B, a.n_groups), dim3(64 * UKV_PAGE16_WAVES), stream);
+      const dim3 grid(a.B, a.n_groups), block(64 * UKV_PAGE16_WAVES);
+      if (a.k_new)
+        hipLaunchKernelGGL((page16_split_kernel<DT, D, true, kDirect>), grid, block, 0, stream, a);
+      else
+        hipLaunchKernelGGL((page16_split_kernel<DT, D, false, kDirect>), grid, block, 0, stream, a);
       return;
     }
     if (a.n_groups <= UKV_PAGE16_WAVES / 2) {
-      auto s = a;
+      DecodeArgs s = a;
       for (s.subs = 2; 2 * s.subs * a.n_groups <= UKV_PAGE16_WAVES;) s.subs *= 2;
-      launch_mode<DT, D, kShared, QF>(s, dim3(a.grid_wgs), dim3(64 * s.subs * a.n_groups), stream);
+      const dim3 grid(a.grid_wgs), block(64 * s.subs * a.n_groups);
+      if (a.k_new)
+        hipLaunchKernelGGL((page16_split_kernel<DT, D, true, kShared>), grid, block, 0, stream, s);
+      else
+        hipLaunchKernelGGL((page16_split_kernel<DT, D, false, kShared>), grid, block, 0, stream, s);
       return;
     }
   }
   const int waves = std::min(UKV_PAGE16_WAVES, a.n_groups);
   const dim3 grid(a.grid_wgs, 1, (a.n_groups + waves - 1) / waves);
-  launch_mode<DT, D, kSplit, QF>(a, grid, dim3(64 * waves), stream);
+  if (a.k_new)
+    hipLaunchKernelGGL((page16_split_kernel<DT, D, true, kSplit>), grid, dim3(64 * waves), 0, stream, a);
+  else
+    hipLaunchKernelGGL((page16_split_kernel<DT, D, false, kSplit>), grid, dim3(64 * waves), 0, stream, a);
 }
 
 template <int DT>
-void launch_combine_dt(const DecodeArgs& a, hipStream_t stream) {
-  const dim3 grid(a.Hq, a.B);
-  const size_t lds = (size_t)(a.grid_wgs + 256 * 4) * sizeof(float);
-  switch (a.D) {
-    case 64: hipLaunchKernelGGL((page16_combine_kernel<DT, 64>), grid, dim3(256), lds, stream, a); break;
-    case 128: hipLaunchKernelGGL((page16_combine_kernel<DT, 128>), grid, dim3(256), lds, stream, a); break;
-    default: hipLaunchKernelGGL((page16_combine_kernel<DT, 256>), grid, dim3(256), lds, stream, a); break;
-  }
-}
-
-void launch_combine(const DecodeArgs& a, int dtype, hipStream_t stream) {
-  if (dtype == UKV_DTYPE_BF16)
-    launch_combine_dt<UKV_DTYPE_BF16>(a, stream);
-  else
-    launch_combine_dt<UKV_DTYPE_F16>(a, stream);
-}
-
-template <int DT, int QF = kCache16>
-bool dispatch_split(const typename SplitArgs<QF>::type& a, hipStream_t stream) {
+bool dispatch_split(const DecodeArgs& a, hipStream_t stream) {
   if (a.n_rep > 16) return false;
   switch (a.D) {
-    case 64: launch_split<DT, 64, QF>(a, stream); return true;
-    case 128: launch_split<DT, 128, QF>(a, stream); return true;
-    case 256: launch_split<DT, 256, QF>(a, stream); return true;
+    case 64: launch_split<DT, 64>(a, stream); return true;
+    case 128: launch_split<DT, 128>(a, stream); return true;
+    case 256: launch_split<DT, 256>(a, stream); return true;
     default: return false;
   }
 }
@@ -1177,72 +720,6 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
 }
 
 }  // namespace
-
-// The decode over the 8-bit cache (arguments checked by the caller): the split kernel where the shape and the
-// alignment allow, else a workgroup for each (sequence, q head).
-int ukv::quant_decode(const QuantAttnArgs& x, int dtype, int format, void* workspace, size_t workspace_bytes,
-                      hipStream_t stream) {
-  const QuantLayer& c = x.c;
-  const int n_groups = (x.Hq + x.n_rep - 1) / x.n_rep;
-  const int64_t codes = c.k_sp | c.k_st | c.k_sh | c.v_sp | c.v_st | c.v_sh;
-  const int64_t exps = c.ks_sp | c.ks_sh | c.ks_sb | c.vs_sp | c.vs_sh | c.vs_sb;
-  auto aligned = [](const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
-  const unsigned wide = (unsigned)x.D / 16;  // bytes of a lane's dims
-  if (!((x.D == 64 || x.D == 128 || x.D == 256) && x.n_rep <= 16 && x.max_blocks > 0 && x.q_st % 8 == 0 &&
-        x.q_sh % 8 == 0 && (codes & (wide - 1)) == 0 && (exps & 3) == 0 && aligned16(x.q) && aligned16(x.out) &&
-        aligned(c.k, wide) && aligned(c.v, wide) && aligned(c.ks, 4) && aligned(c.vs, 4)))
-    return quant_rows_attention(x, x.B, dtype, format, stream);
-  const WorkspaceLayout w = workspace_layout(x.B, x.Hq, x.D, x.max_blocks);
-  if (!workspace || workspace_bytes < w.total || !aligned16(workspace)) return UKV_ERR_WORKSPACE;
-  QuantDecodeArgs a{};
-  a.q = x.q;
-  a.k = reinterpret_cast<const uint16_t*>(c.k);
-  a.v = reinterpret_cast<const uint16_t*>(c.v);
-  a.bt = x.bt;
-  a.lens = x.lens;
-  a.out = x.out;
-  a.q_sb = x.q_st;
-  a.q_sh = x.q_sh;
-  a.k_sp = c.k_sp;
-  a.k_st = c.k_st;
-  a.k_sh = c.k_sh;
-  a.v_sp = c.v_sp;
-  a.v_st = c.v_st;
-  a.v_sh = c.v_sh;
-  a.ks = c.ks;
-  a.vs = c.vs;
-  a.ks_sp = c.ks_sp;
-  a.ks_sh = c.ks_sh;
-  a.ks_sb = c.ks_sb;
-  a.vs_sp = c.vs_sp;
-  a.vs_sh = c.vs_sh;
-  a.vs_sb = c.vs_sb;
-  a.B = x.B;
-  a.Hq = x.Hq;
-  a.n_rep = x.n_rep;
-  a.n_groups = n_groups;
-  a.D = x.D;
-  a.max_blocks = x.max_blocks;
-  a.num_pages = c.num_pages;
-  a.scale = x.scale;
-  a.scale_log2 = x.scale * kLog2e;
-  char* ws = static_cast<char*>(workspace);
-  a.part_o = reinterpret_cast<float*>(ws + w.part_o_off);
-  a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml_off);
-  a.seq_start = reinterpret_cast<int32_t*>(ws + w.seq_off);
-  a.seq_pages = a.seq_start + x.B;
-  a.grid_wgs = launch_wgs(w.wgs, x.B, x.max_blocks, n_groups);
-  a.fixed_shares = env_wgs() > 0;
-  if (dtype == UKV_DTYPE_BF16)
-    format == UKV_CACHE_INT8 ? dispatch_split<UKV_DTYPE_BF16, UKV_CACHE_INT8>(a, stream)
-                             : dispatch_split<UKV_DTYPE_BF16, UKV_CACHE_FP8>(a, stream);
-  else
-    format == UKV_CACHE_INT8 ? dispatch_split<UKV_DTYPE_F16, UKV_CACHE_INT8>(a, stream)
-                             : dispatch_split<UKV_DTYPE_F16, UKV_CACHE_FP8>(a, stream);
-  if (hipGetLastError() != hipSuccess) return UKV_ERR_LAUNCH;
-  if (!direct_shape(x.B, n_groups, x.n_rep, x.D, x.max_blocks)) launch_combine(a, dtype, stream);
-  return hipGetLastError() == hipSuccess ? UKV_OK : UKV_ERR_LAUNCH;
-}
 
 extern "C" int ukv_page16_decode(const void* q, const void* k_cache, const void* v_cache,
                                  const int32_t* block_table, const int32_t* seqlens, void* out, int batch,

@@ -430,5 +430,18 @@ extern "C" int ukv_quant_prefill(const void* q, const void* k, const void* v, co
   if (rc != UKV_OK) return rc;
   // The chunks hold total_q queries, so the longest holds at least total_q / batch of them.
   if ((int64_t)max_chunk * batch < total_q) return UKV_ERR_INVALID_ARGUMENT;
-  return quant_prefill(a, total_q, dtype, format, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  int status = UKV_OK;
+  if (quant_chunk(a, dtype, format, workspace, workspace_bytes, s, status)) return status;
+  return quant_prefill(a, total_q, dtype, format, workspace, workspace_bytes, s);
+}
+
+extern "C" size_t ukv_quant_prefill_workspace_bytes(int batch, int total_q, int max_chunk, int num_q_heads,
+                                                    int num_kv_heads, int head_dim, int n_rep, int max_blocks) {
+  if (batch <= 0 || total_q <= 0 || max_chunk <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || n_rep < 1 ||
+      max_blocks <= 0)
+    return 0;
+  return std::max(quant_chunk_workspace(batch, num_q_heads, n_rep, head_dim, max_chunk, max_blocks),
+                  ukv_paged_prefill_workspace_bytes(batch, total_q, max_chunk, num_q_heads, num_kv_heads, head_dim,
+                                                    n_rep, max_blocks));
 }

@@ -18,13 +18,19 @@ struct QuantAttnArgs {
   float scale;
 };
 
-// page16_decode.hip; the workspace is ukv_page16_workspace_bytes().
+// quant_split.hip; the workspace is ukv_page16_workspace_bytes().
 int quant_decode(const QuantAttnArgs& a, int dtype, int format, void* workspace, size_t workspace_bytes,
                  hipStream_t stream);
 
 // quant_prefill.hip; the workspace (null: none) is ukv_paged_prefill_workspace_bytes().
 int quant_prefill(const QuantAttnArgs& a, int total_q, int dtype, int format, void* workspace, size_t workspace_bytes,
                   hipStream_t stream);
+
+// quant_split.hip: chunks of a few queries. Returns whether the split kernel takes them (with this workspace, of
+// quant_chunk_workspace() bytes), and then the status.
+bool quant_chunk(const QuantAttnArgs& a, int dtype, int format, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream, int& status);
+size_t quant_chunk_workspace(int batch, int hq, int n_rep, int d, int max_chunk, int max_blocks);
 
 int quant_rows_attention(const QuantAttnArgs& a, int rows, int dtype, int format, hipStream_t stream);
 

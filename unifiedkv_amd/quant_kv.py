@@ -243,11 +243,11 @@ def prefill_attention(q: torch.Tensor, layer: QuantLayer, block_table: torch.Ten
     lib = _ext.load()
     width = int(bt.shape[1])
     shape = (B, total_q, mc, Hq, layer.num_heads, D, int(n_rep))
-    need = lib.ukv_paged_prefill_workspace_bytes(*shape, width)
+    need = lib.ukv_quant_prefill_workspace_bytes(*shape, width)
     if need:
         # (a table wider than its sequences: where the host knows the lengths, a call without scratch may do)
         pages = _longest_pages(kv_lens, host_lens)
-        if pages is not None and pages < width and not lib.ukv_paged_prefill_workspace_bytes(*shape, pages):
+        if pages is not None and pages < width and not lib.ukv_quant_prefill_workspace_bytes(*shape, pages):
             need = 0
     ws = None
     if need:
