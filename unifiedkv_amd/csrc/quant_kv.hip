@@ -22,6 +22,9 @@ struct QuantRowsArgs {
   const int32_t* cu;    // [B + 1] first row of each sequence; null: max_chunk rows each
   const int32_t* lens;  // [B] tokens of each sequence with its rows, less lens_add; null: the rows alone
   int lens_add, max_chunk, H, D, max_blocks;
+  int slice;        // eight-dim chunks of a row that a workgroup takes (whole blocks; blockIdx.z: which)
+  float inv_head;   // 1 / those of a head
+  int wide_exps;            // sixteen tokens' exponents are one 16-byte store
 };
 
 // A sequence's rows: `first`.. of the packed ones, `count` of them, at positions `before`.. (64 bits: any length
@@ -77,32 +80,76 @@ template <int DT, int QF> __device__ __forceinline__ uint32_t quantise8(const u3
   return (uint32_t)(e + 127);
 }
 
-// Rows of whole blocks (D a multiple of 32), 16-byte aligned: a thread takes eight dims of a (row, head), K and V.
+// The pages a sequence's rows lie on, one after another for each workgroup of the sequence: rows i0 .. i0 + n - 1 are
+// on page `id` from slot `slot` on.
+template <class F> __device__ __forceinline__ void for_pages(const QuantRowsArgs& a, int b, F f) {
+  const RowSpan s = span_of(a, b);
+  const int64_t begin = max(s.before, (int64_t)0), end = min(s.before + s.count, (int64_t)s.cap);
+  for (int64_t pg = (begin >> 4) + blockIdx.x; 16 * pg < end; pg += gridDim.x) {
+    const int64_t lo = max(begin, 16 * pg);
+    f(page_of(a, s, b, lo), s.first + (int)(lo - s.before), (int)(min(end, 16 * pg + 16) - lo), (int)(lo & 15));
+  }
+}
+// floor(x / n) for x < 2^20 from inv = 1 / n: (x + 1/2) / n is off the next integer by 1/2n at least.
+__device__ __forceinline__ int div_small(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
+
+// Rows of whole blocks (D a multiple of 32), 16-byte aligned: a workgroup takes a page, a thread eight dims of a (row,
+// head) at a time, K and V, kAtOnce loads of both before the first is used. A page's exponents, sixteen tokens
+// together, meet in LDS and go out as 16-byte stores; a part of a page's go out as bytes. Bound: HBM (reads two bytes, writes one).
 template <int DT, int QF>
 __global__ void __launch_bounds__(256) quant_write_kernel(const QuantRowsArgs a) {
-  const int b = blockIdx.y;
-  const RowSpan s = span_of(a, b);
-  const uint32_t per = a.D / 8;
-  const int64_t total = (int64_t)max(s.count, 0) * a.H * per, step = (int64_t)gridDim.x * 256;
-  for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < total; it += step) {
-    const uint32_t c = it % per;
-    const int64_t r = it / per;
-    const int h = (int)(r % a.H), i = (int)(r / a.H);
-    const int64_t pos = s.before + i;
-    const int page = page_of(a, s, b, pos);
-    if (page < 0) continue;  // (the same in a block's four lanes)
-    const u32x4 kx = ld16(a.rows_k + (int64_t)(s.first + i) * a.rk_st + (int64_t)h * a.rk_sh + 8 * c);
-    const u32x4 vx = ld16(a.rows_v + (int64_t)(s.first + i) * a.rv_st + (int64_t)h * a.rv_sh + 8 * c);
-    u32x2 kc, vc;
-    const uint32_t ke = quantise8<DT, QF>(kx, kc), ve = quantise8<DT, QF>(vx, vc);
-    const int64_t slot = pos & 15;
-    *reinterpret_cast<u32x2*>(const_cast<uint8_t*>(a.c.k) + page * a.c.k_sp + slot * a.c.k_st + h * a.c.k_sh + 8 * c) = kc;
-    *reinterpret_cast<u32x2*>(const_cast<uint8_t*>(a.c.v) + page * a.c.v_sp + slot * a.c.v_st + h * a.c.v_sh + 8 * c) = vc;
-    if (c % 4 == 0) {
-      const_cast<uint8_t*>(a.c.ks)[page * a.c.ks_sp + h * a.c.ks_sh + (c / 4) * a.c.ks_sb + slot] = (uint8_t)ke;
-      const_cast<uint8_t*>(a.c.vs)[page * a.c.vs_sp + h * a.c.vs_sh + (c / 4) * a.c.vs_sb + slot] = (uint8_t)ve;
+  constexpr int kAtOnce = 4;
+  extern __shared__ __attribute__((aligned(16))) uint8_t exps[];  // [K, V][blocks of the slice][16]
+  const int per = a.D / 8, x0 = blockIdx.z * a.slice, row = min(a.slice, a.H * per - x0), blocks = row / 4;
+  const float inv_row = 1.f / (float)row;
+  for_pages(a, blockIdx.y, [&](int64_t page, int r0, int n, int slot0) {
+    const bool together = n == 16 && a.wide_exps;  // (uniform, as is page < 0)
+    uint8_t* kp = const_cast<uint8_t*>(a.c.k) + page * a.c.k_sp;
+    uint8_t* vp = const_cast<uint8_t*>(a.c.v) + page * a.c.v_sp;
+    uint8_t* ke = const_cast<uint8_t*>(a.c.ks) + page * a.c.ks_sp;
+    uint8_t* ve = const_cast<uint8_t*>(a.c.vs) + page * a.c.vs_sp;
+    for (int base = threadIdx.x; base < n * row; base += 256 * kAtOnce) {
+      u32x4 kx[kAtOnce], vx[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int it = min(base + 256 * j, n * row - 1), i = div_small(it, inv_row), x = x0 + it - i * row;
+        const int h = div_small(x, a.inv_head), c = x - h * per;
+        const int64_t r = r0 + i;
+        kx[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.rows_k + r * a.rk_st + h * a.rk_sh + 8 * c));
+        vx[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.rows_v + r * a.rv_st + h * a.rv_sh + 8 * c));
+      }
+      if (page < 0) return;  // (after the rows are asked for, which its id would keep waiting)
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int it = base + 256 * j;
+        if (it >= n * row) break;  // (the same in a block's four lanes)
+        const int i = div_small(it, inv_row), x = x0 + it - i * row, h = div_small(x, a.inv_head), c = x - h * per;
+        const int64_t slot = slot0 + i;
+        u32x2 kc, vc;
+        const uint32_t k_exp = quantise8<DT, QF>(kx[j], kc), v_exp = quantise8<DT, QF>(vx[j], vc);
+        *reinterpret_cast<u32x2*>(kp + slot * a.c.k_st + h * a.c.k_sh + 8 * c) = kc;
+        *reinterpret_cast<u32x2*>(vp + slot * a.c.v_st + h * a.c.v_sh + 8 * c) = vc;
+        if ((c & 3) == 0) {
+          if (together) {
+            exps[(x - x0) * 4 + slot] = (uint8_t)k_exp;
+            exps[(4 * blocks + x - x0) * 4 + slot] = (uint8_t)v_exp;
+          } else {
+            ke[h * a.c.ks_sh + (c / 4) * a.c.ks_sb + slot] = (uint8_t)k_exp;
+            ve[h * a.c.vs_sh + (c / 4) * a.c.vs_sb + slot] = (uint8_t)v_exp;
+          }
+        }
+      }
     }
-  }
+    if (!together) return;
+    __syncthreads();
+    for (int y = threadIdx.x; y < 2 * blocks; y += 256) {
+      const bool is_v = y >= blocks;
+      const int x = x0 / 4 + (is_v ? y - blocks : y), h = div_small(4 * x, a.inv_head), blk = x - h * (per / 4);
+      uint8_t* to = is_v ? ve + h * a.c.vs_sh + blk * a.c.vs_sb : ke + h * a.c.ks_sh + blk * a.c.ks_sb;
+      *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(exps + 16 * y);
+    }
+    __syncthreads();  // read before the next page's
+  });
 }
 
 // Any row: a thread takes a block of one (row, head) of K or V.
@@ -141,34 +188,65 @@ __global__ void __launch_bounds__(256) quant_write_any_kernel(const QuantRowsArg
   }
 }
 
-// Rows back from the cache: a thread takes eight dims of a (row, head), K and V. A row without a page reads as zeros.
+// Rows back from the cache, cut as the write is. A row without a page reads as zeros; rows outside the table are no
+// part of any page, and the workgroups share them at the end.
 template <int DT, int QF>
 __global__ void __launch_bounds__(256) quant_read_kernel(const QuantRowsArgs a) {
-  const int b = blockIdx.y;
-  const RowSpan s = span_of(a, b);
-  const uint32_t per = a.D / 8;
-  const int64_t total = (int64_t)max(s.count, 0) * a.H * per, step = (int64_t)gridDim.x * 256;
-  for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < total; it += step) {
-    const uint32_t c = it % per;
-    const int64_t r = it / per;
-    const int h = (int)(r % a.H), i = (int)(r / a.H);
-    const int64_t pos = s.before + i;
-    const int page = page_of(a, s, b, pos);
-    u32x4 kx = {0u, 0u, 0u, 0u}, vx = kx;
-    if (page >= 0) {
-      const int64_t slot = pos & 15;
-      const u32x2 kc = *reinterpret_cast<const u32x2*>(a.c.k + page * a.c.k_sp + slot * a.c.k_st + h * a.c.k_sh + 8 * c);
-      const u32x2 vc = *reinterpret_cast<const u32x2*>(a.c.v + page * a.c.v_sp + slot * a.c.v_st + h * a.c.v_sh + 8 * c);
-      const float ks = quant_scale(a.c.ks[page * a.c.ks_sp + h * a.c.ks_sh + (c / 4) * a.c.ks_sb + slot]);
-      const float vs = quant_scale(a.c.vs[page * a.c.vs_sp + h * a.c.vs_sh + (c / 4) * a.c.vs_sb + slot]);
-      const u32x2 k0 = quant_elems4<QF, DT>(kc[0], ks), k1 = quant_elems4<QF, DT>(kc[1], ks);
-      const u32x2 v0 = quant_elems4<QF, DT>(vc[0], vs), v1 = quant_elems4<QF, DT>(vc[1], vs);
-      kx = u32x4{k0[0], k0[1], k1[0], k1[1]};
-      vx = u32x4{v0[0], v0[1], v1[0], v1[1]};
+  constexpr int kAtOnce = 4;
+  const int per = a.D / 8, x0 = blockIdx.z * a.slice, row = min(a.slice, a.H * per - x0);
+  const float inv_row = 1.f / (float)row;
+  auto store = [&](int64_t r, int h, int c, const u32x4& k, const u32x4& v) {
+    __builtin_nontemporal_store(k, reinterpret_cast<u32x4*>(a.rows_k + r * a.rk_st + h * a.rk_sh + 8 * c));
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(a.rows_v + r * a.rv_st + h * a.rv_sh + 8 * c));
+  };
+  for_pages(a, blockIdx.y, [&](int64_t page, int r0, int n, int slot0) {
+    const bool ok = page >= 0;  // (uniform)
+    const int64_t at = ok ? page : 0;
+    const uint8_t *kp = a.c.k + at * a.c.k_sp, *vp = a.c.v + at * a.c.v_sp;
+    const uint8_t *ke = a.c.ks + at * a.c.ks_sp, *ve = a.c.vs + at * a.c.vs_sp;
+    for (int base = threadIdx.x; base < n * row; base += 256 * kAtOnce) {
+      u32x2 kc[kAtOnce] = {}, vc[kAtOnce] = {};
+      uint32_t k_exp[kAtOnce] = {}, v_exp[kAtOnce] = {};
+      if (ok) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int it = min(base + 256 * j, n * row - 1), i = div_small(it, inv_row), x = x0 + it - i * row;
+          const int h = div_small(x, a.inv_head), c = x - h * per;
+          const int64_t slot = slot0 + i;
+          kc[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kp + slot * a.c.k_st + h * a.c.k_sh + 8 * c));
+          vc[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vp + slot * a.c.v_st + h * a.c.v_sh + 8 * c));
+          k_exp[j] = ke[h * a.c.ks_sh + (c >> 2) * a.c.ks_sb + slot];
+          v_exp[j] = ve[h * a.c.vs_sh + (c >> 2) * a.c.vs_sb + slot];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int it = base + 256 * j;
+        if (it >= n * row) break;
+        const int i = div_small(it, inv_row), x = x0 + it - i * row, h = div_small(x, a.inv_head), c = x - h * per;
+        u32x4 k = {0u, 0u, 0u, 0u}, v = k;
+        if (ok) {
+          const float ks = quant_scale(k_exp[j]), vs = quant_scale(v_exp[j]);
+          const u32x2 k0 = quant_elems4<QF, DT>(kc[j][0], ks), k1 = quant_elems4<QF, DT>(kc[j][1], ks);
+          const u32x2 v0 = quant_elems4<QF, DT>(vc[j][0], vs), v1 = quant_elems4<QF, DT>(vc[j][1], vs);
+          k = u32x4{k0[0], k0[1], k1[0], k1[1]};
+          v = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        }
+        store(r0 + i, h, c, k, v);
+      }
     }
-    *reinterpret_cast<u32x4*>(a.rows_k + (int64_t)(s.first + i) * a.rk_st + (int64_t)h * a.rk_sh + 8 * c) = kx;
-    *reinterpret_cast<u32x4*>(a.rows_v + (int64_t)(s.first + i) * a.rv_st + (int64_t)h * a.rv_sh + 8 * c) = vx;
-  }
+  });
+  const RowSpan s = span_of(a, blockIdx.y);
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  auto clear = [&](int64_t from, int64_t to) {  // the sequence's rows from .. to - 1
+    for (int64_t i = from + blockIdx.x; i < to; i += gridDim.x)
+      for (int x = x0 + threadIdx.x; x < x0 + row; x += 256) {
+        const int h = div_small(x, a.inv_head);
+        store(s.first + i, h, x - h * per, zero, zero);
+      }
+  };
+  clear(0, min((int64_t)s.count, -s.before));                // positions below zero
+  clear(max((int64_t)0, s.cap - s.before), s.count);         // positions past the table
 }
 
 // Any row: a thread takes one element of K and V.
@@ -281,26 +359,37 @@ namespace {
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// Whether a thread's eight dims are one 16-byte access of the rows and one 8-byte access of the codes.
+// Whether a thread's eight dims are one 16-byte access of the rows and one 8-byte access of the codes, and a page's
+// exponents fit LDS (32 KB).
 bool wide_rows(const QuantRowsArgs& a) {
   const int64_t rows = a.rk_st | a.rk_sh | a.rv_st | a.rv_sh;
   const int64_t codes = a.c.k_sp | a.c.k_st | a.c.k_sh | a.c.v_sp | a.c.v_st | a.c.v_sh;
-  return a.D % kQuantBlock == 0 && ((rows | codes) & 7) == 0 && aligned(a.rows_k, 16) && aligned(a.rows_v, 16) &&
+  return a.D % kQuantBlock == 0 && a.H * a.D <= 32768 && ((rows | codes) & 7) == 0 && aligned(a.rows_k, 16) && aligned(a.rows_v, 16) &&
          aligned(a.c.k, 8) && aligned(a.c.v, 8);
 }
 
+constexpr int kSlice = 64;
 constexpr int64_t kMostWgs = 1 << 16;  // (longer calls: a workgroup takes several spans of its sequence)
 
-template <int DT, int QF> void launch_rows(const QuantRowsArgs& a, int batch, bool write, hipStream_t stream) {
-  const bool wide = wide_rows(a);
+template <int DT, int QF> void launch_rows(QuantRowsArgs a, int batch, bool write, hipStream_t stream) {
   const int blocks = (a.D + kQuantBlock - 1) / kQuantBlock;
-  const int64_t items = (int64_t)a.max_chunk * a.H * (wide ? a.D / 8 : write ? blocks : a.D);
+  if (wide_rows(a)) {
+    // A workgroup a page (a chunk of n rows touches (n + 14) / 16 + 1 at most), or, where these are fewer than eight a
+    // CU, a few heads of one: 8192 tokens of 8 x 128 dims written and read back in 24.4 us with two slices, 26.5 with
+    // one or four.
+    const unsigned x = (unsigned)std::min<int64_t>(((int64_t)a.max_chunk + 14) / 16 + 1, kMostWgs);
+    const int row = a.H * (a.D / 8);
+    a.slice = (int64_t)x * batch < 2048 ? std::min(row, kSlice) : row;
+    const dim3 grid(x, batch, (row + a.slice - 1) / a.slice);
+    if (write)
+      hipLaunchKernelGGL((quant_write_kernel<DT, QF>), grid, dim3(256), 8 * a.slice, stream, a);
+    else
+      hipLaunchKernelGGL((quant_read_kernel<DT, QF>), grid, dim3(256), 0, stream, a);
+    return;
+  }
+  const int64_t items = (int64_t)a.max_chunk * a.H * (write ? blocks : a.D);
   const unsigned x = (unsigned)std::min<int64_t>((items + 255) / 256, kMostWgs);
-  if (wide && write)
-    hipLaunchKernelGGL((quant_write_kernel<DT, QF>), dim3(x, batch), dim3(256), 0, stream, a);
-  else if (wide)
-    hipLaunchKernelGGL((quant_read_kernel<DT, QF>), dim3(x, batch), dim3(256), 0, stream, a);
-  else if (write)
+  if (write)
     hipLaunchKernelGGL((quant_write_any_kernel<DT, QF>), dim3(x, batch, 2), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((quant_read_any_kernel<DT, QF>), dim3(x, batch), dim3(256), 0, stream, a);
@@ -334,6 +423,9 @@ int rows_call(bool write, const void* k, const void* v, const void* ks, const vo
   a.H = num_heads;
   a.D = head_dim;
   a.max_blocks = max_blocks;
+  a.inv_head = 8.f / (float)head_dim;
+  const int64_t exps = a.c.ks_sp | a.c.ks_sh | a.c.ks_sb | a.c.vs_sp | a.c.vs_sh | a.c.vs_sb;
+  a.wide_exps = (exps & 15) == 0 && aligned(ks, 16) && aligned(vs, 16);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == UKV_DTYPE_BF16)
     format == UKV_CACHE_INT8 ? launch_rows<UKV_DTYPE_BF16, UKV_CACHE_INT8>(a, batch, write, s)

@@ -34,7 +34,6 @@ struct QuantSplitArgs : DecodeArgs {
   int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
   const int32_t* cu;  // chunks: [B + 1] first query row of each sequence
   int max_chunk;      // queries a sequence at most (decode: 1)
-  int passes;         // workgroups (blockIdx.y) that share a share's columns
 };
 
 typedef const __attribute__((address_space(1))) uint8_t global_u8;
@@ -104,8 +103,7 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
   const int subs = DIRECT ? UKV_PAGE16_WAVES : SHARED ? a.subs : 1;
   const int g = DIRECT ? (int)blockIdx.y : SHARED ? wv - sub * a.n_groups : blockIdx.z * (blockDim.x >> 6) + wv;
   if (!SHARED && g >= a.n_groups) return;  // whole wave leaves; only SHARED has barriers below
-  const int pass = CHUNK ? blockIdx.y : 0;
-  const bool writer = blockIdx.x == 0 && blockIdx.z == 0 && pass == 0 && wv == 0;
+  const bool writer = blockIdx.x == 0 && blockIdx.z == 0 && wv == 0;
 
   // This workgroup's share of the pages: pages x0 .. x1 - 1 of the batch's list, from page x0 - s_first of sequence
   // b_first on (page16_decode.hip has the reasons). w: the share's number.
@@ -200,8 +198,8 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
     s.pa = __builtin_amdgcn_readfirstlane(pa);
     s.n_pages = __builtin_amdgcn_readfirstlane(min(((s.L + 15) >> 4) - pa, most));
     s.n_mine = SHARED ? __builtin_amdgcn_readfirstlane(max(0, s.n_pages - sub + subs - 1) / subs) : s.n_pages;
-    if constexpr (CHUNK)  // no query of the sequence in this pass's columns: its pages are not read
-      if (pass * CB * 16 >= (a.cu[s.b + 1] - a.cu[s.b]) * a.n_rep) s.n_mine = 0;
+    if constexpr (CHUNK)
+      if (a.cu[s.b + 1] <= a.cu[s.b]) s.n_mine = 0;  // no query: the pages are not read
     return s;
   };
   auto page_at = [&](const Segment& s, int i) -> int { return SHARED ? s.pa + sub + i * subs : s.pa + i; };
@@ -411,9 +409,9 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
       all_see = s.L - C + 1;
     }
     // Column x of block cb: its query and q head.
-    auto col_query = [&](int cb, int x) -> int { return CHUNK ? ((pass * CB + cb) * 16 + x) / a.n_rep : 0; };
+    auto col_query = [&](int cb, int x) -> int { return CHUNK ? (cb * 16 + x) / a.n_rep : 0; };
     auto col_head = [&](int cb, int x) -> int {
-      return g * a.n_rep + (CHUNK ? ((pass * CB + cb) * 16 + x) % a.n_rep : x);
+      return g * a.n_rep + (CHUNK ? (cb * 16 + x) % a.n_rep : x);
     };
     auto col_live = [&](int cb, int x) -> bool {
       return (CHUNK ? col_query(cb, x) < min(C, a.max_chunk) : x < a.n_rep) && col_head(cb, x) < a.Hq;
@@ -582,11 +580,11 @@ template <int DT, int D, int QF> void launch_decode(const QuantSplitArgs& a, hip
 template <int DT, int D, int CB, int QF> void launch_chunk(const QuantSplitArgs& a, hipStream_t stream) {
   const int waves = std::min(UKV_PAGE16_WAVES, a.n_groups);
   if (a.n_groups <= UKV_PAGE16_WAVES / 2)
-    hipLaunchKernelGGL((quant_split_kernel<DT, D, CB, true, kShared, QF>), dim3(a.grid_wgs, a.passes),
+    hipLaunchKernelGGL((quant_split_kernel<DT, D, CB, true, kShared, QF>), dim3(a.grid_wgs),
                        dim3(64 * a.subs * a.n_groups), 0, stream, a);
   else
     hipLaunchKernelGGL((quant_split_kernel<DT, D, CB, true, kSplit, QF>),
-                       dim3(a.grid_wgs, a.passes, (a.n_groups + waves - 1) / waves), dim3(64 * waves), 0, stream, a);
+                       dim3(a.grid_wgs, 1, (a.n_groups + waves - 1) / waves), dim3(64 * waves), 0, stream, a);
   const size_t lds = (size_t)(a.grid_wgs + 256 * 4) * sizeof(float);
   hipLaunchKernelGGL((quant_chunk_combine_kernel<DT, D>), dim3(a.max_chunk * a.Hq, a.B), dim3(256), lds, stream, a);
 }
@@ -656,7 +654,6 @@ int launch(const QuantAttnArgs& x, bool chunk, const WorkspaceLayout& w, int dty
   a.max_blocks = x.max_blocks;
   a.num_pages = c.num_pages;
   a.max_chunk = chunk ? x.max_chunk : 1;
-  a.passes = chunk ? (x.max_chunk * x.n_rep + 31) / 32 : 1;
   a.scale = x.scale;
   a.scale_log2 = x.scale * kLog2e;
   for (a.subs = 2; 2 * a.subs * a.n_groups <= UKV_PAGE16_WAVES;) a.subs *= 2;  // (where the kernel shares heads)
@@ -678,11 +675,16 @@ int launch(const QuantAttnArgs& x, bool chunk, const WorkspaceLayout& w, int dty
   return hipGetLastError() == hipSuccess ? UKV_OK : UKV_ERR_LAUNCH;
 }
 
-// Chunks the split kernel takes: a few columns, so that a pass over the keys for every 32 of them costs less than the
-// tiled kernel's workgroups, whose waves each hold 32 or 48.
-constexpr int kMostPasses = 2;
-bool chunk_shape(int max_chunk, int n_rep, int head_dim) {
-  return (head_dim == 64 || head_dim == 128) && n_rep <= 32 && (int64_t)max_chunk * n_rep <= 32 * kMostPasses;
+// Chunks the split kernel takes: up to two column blocks a wave. One block always pays against the tiled kernel, whose
+// workgroups hold 256 columns and more: two queries a sequence on 32/8 heads, 16 sequences of 100-600 tokens 17.8 us
+// against 22.5, 32 of 1-4K 44 against 96, one of 32K 32 against 59. Two need keys enough for the shares, four pages a CU:
+// eight queries 66 against 98 and 41 against 60 us behind the longer ones, but 32 against 24 behind 100-600 tokens and 27
+// against 24 for four of 300-1500. (A second pass over the keys for up to 64 columns paid behind sixteen sequences of
+// 4-32K, 236 us against 348, not behind one of 32K, 66 against 61, or 32 of 1-4K, 120 against 100.)
+bool chunk_shape(int batch, int max_chunk, int n_rep, int head_dim, int max_blocks) {
+  const int64_t columns = (int64_t)max_chunk * n_rep;
+  return (head_dim == 64 || head_dim == 128) &&
+         (columns <= 16 || (columns <= 32 && (int64_t)batch * max_blocks >= 4 * device_cu_count()));
 }
 
 WorkspaceLayout chunk_layout(int batch, int hq, int d, int max_chunk, int max_blocks) {
@@ -702,12 +704,12 @@ int quant_decode(const QuantAttnArgs& x, int dtype, int format, void* workspace,
 }
 
 size_t quant_chunk_workspace(int batch, int hq, int n_rep, int d, int max_chunk, int max_blocks) {
-  return chunk_shape(max_chunk, n_rep, d) ? chunk_layout(batch, hq, d, max_chunk, max_blocks).total : 0;
+  return chunk_shape(batch, max_chunk, n_rep, d, max_blocks) ? chunk_layout(batch, hq, d, max_chunk, max_blocks).total : 0;
 }
 
 bool quant_chunk(const QuantAttnArgs& x, int dtype, int format, void* workspace, size_t workspace_bytes,
                  hipStream_t stream, int& status) {
-  if (!chunk_shape(x.max_chunk, x.n_rep, x.D) || !split_layout(x)) return false;
+  if (!chunk_shape(x.B, x.max_chunk, x.n_rep, x.D, x.max_blocks) || !split_layout(x)) return false;
   const WorkspaceLayout w = chunk_layout(x.B, x.Hq, x.D, x.max_chunk, x.max_blocks);
   if (!workspace || workspace_bytes < w.total || !aligned16(workspace) || x.B > 65535) return false;
   status = launch(x, true, w, dtype, format, workspace, stream);

@@ -44,28 +44,29 @@ class QuantLayer:
                  "strides", "pointers")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        shape = tuple(k.shape)
+        # (each attribute is read once: a program without a pool may build one per call, 3 us)
+        shape, dtype, dev = k.shape, k.dtype, k.device
         if len(shape) != 4 or shape[1] != 16:
             _refuse("cache")
-        if k.dtype not in _FORMAT_CODES or v.dtype != k.dtype:
+        code = _FORMAT_CODES.get(dtype)
+        if code is None or v.dtype != dtype:
             _refuse("cache_dtype")
         N, _, H, D = shape
-        if tuple(v.shape) != shape:
+        if v.shape != shape:
             _refuse("v_cache")
         want = (N, H, -(-D // QUANT_BLOCK), 16)
-        if tuple(k_scale.shape) != want or tuple(v_scale.shape) != want:
+        if k_scale.shape != want or v_scale.shape != want:
             _refuse("scale")
         if k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8:
             _refuse("scale_dtype")
         ks, vs, kss, vss = k.stride(), v.stride(), k_scale.stride(), v_scale.stride()
         if ks[3] != 1 or vs[3] != 1 or kss[3] != 1 or vss[3] != 1:
             _refuse("cache_stride")
-        dev = k.device
         if v.device != dev or k_scale.device != dev or v_scale.device != dev:
             raise RuntimeError("quant_kv_unavailable:device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.num_heads, self.head_dim = N, H, D
-        self.format_code = _FORMAT_CODES[k.dtype]
+        self.format_code = code
         self.device = dev
         self.strides = _ext.i64_tuple(ks[:3] + vs[:3] + kss[:3] + vss[:3])
         self.pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
@@ -73,7 +74,8 @@ class QuantLayer:
 
 def _check_rows(layer: QuantLayer, k: torch.Tensor, v: torch.Tensor) -> None:
     """K and V rows [total, H, D] of one 16-bit type on the cache's GPU."""
-    if k.dim() != 3 or v.shape != k.shape or tuple(k.shape[1:]) != (layer.num_heads, layer.head_dim):
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[1] != layer.num_heads or shape[2] != layer.head_dim:
         _refuse("rows")
     if k.dtype not in _DTYPE_CODES or v.dtype != k.dtype:
         _refuse("dtype")
@@ -84,8 +86,11 @@ def _check_rows(layer: QuantLayer, k: torch.Tensor, v: torch.Tensor) -> None:
 
 def _check_device(layer: QuantLayer, *tensors: torch.Tensor) -> None:
     dev = layer.device
-    if dev.type != "cuda" or any(t.device != dev for t in tensors):
+    if dev.type != "cuda":
         raise RuntimeError("quant_kv_unavailable:device")
+    for t in tensors:
+        if t.device != dev:
+            raise RuntimeError("quant_kv_unavailable:device")
 
 
 def _check(code: int, layer: QuantLayer) -> None:
@@ -96,8 +101,8 @@ def _check(code: int, layer: QuantLayer) -> None:
 
 
 def _batch(cu, lens, table) -> int:
-    B = int(lens.numel())
-    if table.dim() != 2 or int(table.shape[0]) != B or (cu is not None and int(cu.numel()) != B + 1):
+    B, shape = lens.numel(), table.shape
+    if len(shape) != 2 or shape[0] != B or (cu is not None and cu.numel() != B + 1):
         _refuse("batch")
     return B
 
