@@ -339,11 +339,14 @@ template <> struct PrefillSplit<UKV_DTYPE_F16> {
 // for obs_rows_finish_kernel.
 //   QF     the pages are 8-bit codes: a thread's chunk is eight codes and their exponent byte, which its store
 //          makes the values that they are exactly, K in the queries' type, V in that of P.V's operands. From LDS on
-//          the tile is a 16-bit pool's.
+//          the tile is a 16-bit pool's, but that FINE stands for the columns' layout alone: P is one fp16 number (11
+//          significant bits beside codes of four to eight), which saves the third of the matrix instructions that
+//          the low parts take, and their registers.
 template <int DT, int D, int WAVES, int CB, bool FINE, bool PARTS, int QF>
 __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& a, const int b, const int g,
                                              const int c0, const int part, const int np, PrefillLds<D>& lds) {
   constexpr bool QUANT = QF != kCache16;
+  constexpr bool TWO = FINE && !QUANT;  // weights in two parts
   constexpr int STEPS = D / 32;
   constexpr int NE = D / 16;  // output tiles of 16 dims
   constexpr int NT = 64 * WAVES;
@@ -353,9 +356,9 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
   // A thread loads one 16-byte chunk of K and one of V per tile or, HALF (D = 64), one of either: the
   // lower half of the waves takes K.
   constexpr bool HALF = 2 * TK * CH == NT;
-  constexpr int PVT = FINE ? DT : (int)UKV_DTYPE_F16;  // type of the P.V operands
+  constexpr int PVT = TWO ? DT : (int)UKV_DTYPE_F16;  // type of the P.V operands
   constexpr float kTau = 8.f;
-  constexpr float kLift = FINE ? PrefillSplit<DT>::kLift : 0.f;
+  constexpr float kLift = TWO ? PrefillSplit<DT>::kLift : 0.f;
   constexpr bool kConvert = DT == UKV_DTYPE_BF16 && !FINE && !QUANT;  // the loader converts V to fp16
   static_assert(HALF || TK * CH == NT, "loader mapping");
   auto& k_s = lds.k_s;
@@ -561,7 +564,8 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
     if constexpr (HALF) {
       clear_junk(r.k, r.ke);
       uint16_t* dst = half_v ? &v_s[slot][lds_row][8 * lds_ch] : &k_s[slot][lds_row][8 * lds_ch];
-      *reinterpret_cast<u32x4*>(dst) = widen(r.k, r.ke, k_type);
+      if (DT == PVT || !half_v) *reinterpret_cast<u32x4*>(dst) = widen(r.k, r.ke, k_type);
+      else *reinterpret_cast<u32x4*>(dst) = widen(r.k, r.ke, v_type);
     } else {
       clear_junk(r.v, r.ve);
       *reinterpret_cast<u32x4*>(&k_s[slot][lds_row][8 * lds_ch]) = widen(r.k, r.ke, k_type);
@@ -648,7 +652,7 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
     // 2^8: the packed fp16 P is checked (non-negative fp16 bit patterns order
     // like their values, and inf and NaN lie above), and a column block whose
     // max moved is rescaled and its P recomputed.
-    u32x4 pa[CB], pl[FINE ? CB : 1];  // pl: FINE's low parts
+    u32x4 pa[CB], pl[TWO ? CB : 1];  // pl: the low parts
     auto exp_pack = [&](int cb) {
       float p[2][4];
 #pragma unroll
@@ -656,7 +660,7 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           p[kb][r] = fast_exp2(__builtin_fmaf(sacc[kb][cb][r], sl2, kLift != 0.f ? kLift - m_ref[cb] : -m_ref[cb]));
-      if constexpr (FINE) {
+      if constexpr (TWO) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t hi, lo;
@@ -701,7 +705,7 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) exp_pack(cb);
       bool moved;
-      if constexpr (FINE) {
+      if constexpr (TWO) {
         // (non-negative 16-bit float patterns order like their values; inf and NaN lie above)
         u16x2 mx = {0, 0};
 #pragma unroll
@@ -739,7 +743,7 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
     }
     // FINE holds it through its twice as many P.V MFMAs: 4 x 512 queries on 28/4 heads 310 against
     // 317 us (313 without it at all).
-    if constexpr (!FINE) __builtin_amdgcn_s_setprio(0);
+    if constexpr (!TWO) __builtin_amdgcn_s_setprio(0);
     // P.V: the B operand of output tile e (dims 16e .. 16e + 15) holds, in lane
     // (i16, kg), dim 16e + i16 of keys 4kg..4kg+3 and 16+4kg..16+4kg+3 (the
     // key order of P's A operand). ds_read_b64_tr_b16 builds it from row-major
@@ -753,17 +757,17 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
       const u32x4 bv = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) o[cb][e] = mfma16x16x32<PVT>(pa[cb], bv, o[cb][e]);
-      if constexpr (FINE)
+      if constexpr (TWO)
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) o[cb][e] = mfma16x16x32<PVT>(pl[cb], bv, o[cb][e]);
     }
-    if constexpr (FINE) __builtin_amdgcn_s_setprio(0);
+    if constexpr (TWO) __builtin_amdgcn_s_setprio(0);
     // Denominators: the same P against a ones operand.
-    constexpr uint32_t kOnes = FINE ? PrefillSplit<DT>::kOnes : 0x3C003C00u;
+    constexpr uint32_t kOnes = TWO ? PrefillSplit<DT>::kOnes : 0x3C003C00u;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       lacc[cb] = mfma16x16x32<PVT>(pa[cb], u32x4{kOnes, kOnes, kOnes, kOnes}, lacc[cb]);
-      if constexpr (FINE) lacc[cb] = mfma16x16x32<PVT>(pl[cb], u32x4{kOnes, kOnes, kOnes, kOnes}, lacc[cb]);
+      if constexpr (TWO) lacc[cb] = mfma16x16x32<PVT>(pl[cb], u32x4{kOnes, kOnes, kOnes, kOnes}, lacc[cb]);
     }
   };
 
@@ -825,7 +829,7 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
   }
 
   // (QUANT: where holding them left no register for the scalar spills; in the other instances reading them again did)
-  const auto& e = PARTS || (QUANT && D == 128 && DT == UKV_DTYPE_BF16) ? args_again<typename TileArgs<QF>::type>() : a;
+  const auto& e = PARTS || (QUANT && D == 128 && DT == UKV_DTYPE_BF16 && !FINE) ? args_again<typename TileArgs<QF>::type>() : a;
   // A V the matrix cores got wrong anywhere in this workgroup's keys: its columns again on the fp32
   // fallback.
   bool redo_mine = false;
@@ -1020,7 +1024,7 @@ __device__ __forceinline__ bool locate_item(int start, int end, int n, int nl, i
 // accumulators, queries and weights (in two parts for FINE) stay in 256 VGPRs. 64-dim heads are FINE, and
 // two blocks of theirs fit the 128 VGPRs that paged_prefill_kernel asks for at D = 64: two workgroups
 // then share a CU and cover each other's first loads (one 96-token prompt 7.5 us against 11.6).
-constexpr int wide_blocks(bool fine) { return fine ? 2 : 3; }
+constexpr int wide_blocks(bool fine, int head_dim, bool quant) { return (quant ? head_dim == 64 : fine) ? 2 : 3; }
 
 // The range of work items [start, end) of a launch's n_items items that XCD xcd runs: dispatch
 // is round-robin over the 8 XCDs, so the workgroups with blockIdx.x % 8 == xcd run there, and
@@ -1052,7 +1056,7 @@ template <int DT, int D, int WAVES, bool FINE, bool PARTS, int QF = kCache16>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
 paged_prefill_kernel(const typename TileArgs<QF>::type a) {
   __shared__ PrefillLds<D> lds;
-  constexpr int CB3 = wide_blocks(FINE), CB2 = CB3 - 1;
+  constexpr int CB3 = wide_blocks(FINE, D, QF != kCache16), CB2 = CB3 - 1;
   int n3 = a.n3, n2 = a.n2;
   int start, end, pair, j, part = 0, np = 1;
   const bool parts = PARTS && any_in_parts(a);
@@ -1140,9 +1144,9 @@ bool tiled_shape(int head_dim, int n_rep) { return (head_dim == 128 || head_dim 
 bool fine_shape(int head_dim, int n_rep) { return head_dim != 128 || 16 % n_rep != 0; }
 
 BlockPlan plan_for(int batch, int64_t rows, int max_chunk, int n_groups, int head_dim, int n_rep, int max_blocks,
-                   bool parts) {
+                   bool parts, bool quant) {
   constexpr int W = UKV_PREFILL_WAVES, tile_pages = kTileKeys / 16;
-  const int cb3 = wide_blocks(fine_shape(head_dim, n_rep));
+  const int cb3 = wide_blocks(fine_shape(head_dim, n_rep), head_dim, quant);
   PlanShape f{};
   f.max_cols = (int64_t)max_chunk * n_rep;
   f.pairs = (int64_t)n_groups * batch;
@@ -1169,12 +1173,13 @@ constexpr size_t kMaxPartBytes = size_t(512) << 20;
 
 // The call's block plan, key parts and partials into `a`, whose other fields are set; returns the tiled launch's
 // workgroups. The caller sizes the workspace by the same plan; a smaller one runs without parts.
-int64_t plan_launch(PrefillArgs& a, int total_q, void* workspace, size_t workspace_bytes) {
+int64_t plan_launch(PrefillArgs& a, int total_q, bool quant, void* workspace, size_t workspace_bytes) {
   const int64_t pairs = (int64_t)a.n_groups * a.B, rows = (int64_t)total_q * a.Hq;
-  BlockPlan plan = plan_for(a.B, rows, a.max_chunk, a.n_groups, a.D, a.n_rep, a.max_blocks, workspace != nullptr);
+  BlockPlan plan = plan_for(a.B, rows, a.max_chunk, a.n_groups, a.D, a.n_rep, a.max_blocks, workspace != nullptr,
+                            quant);
   if (plan.parts > 1 && (part_bytes(plan.parts, rows, a.D) > workspace_bytes || (rows + 7) / 8 > INT32_MAX ||
                          (reinterpret_cast<uintptr_t>(workspace) & 15u)))
-    plan = plan_for(a.B, rows, a.max_chunk, a.n_groups, a.D, a.n_rep, a.max_blocks, false);
+    plan = plan_for(a.B, rows, a.max_chunk, a.n_groups, a.D, a.n_rep, a.max_blocks, false, quant);
   a.n3 = plan.n3;
   a.n2 = plan.n2;
   a.n_parts = plan.parts;
@@ -1194,6 +1199,20 @@ int64_t plan_launch(PrefillArgs& a, int total_q, void* workspace, size_t workspa
   // at least half as wide as wide ones.)
   const int64_t items = pairs * (a.n3 + a.n2);
   return plan.parts > 1 ? 8 * ((items * plan.parts + 7) / 8) : items;
+}
+
+// What a call takes to run in parts (0: it runs in one).
+size_t parts_workspace(int batch, int total_q, int max_chunk, int num_q_heads, int num_kv_heads, int head_dim,
+                       int n_rep, int max_blocks, bool quant) {
+  if (batch <= 0 || total_q <= 0 || max_chunk <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || n_rep < 1 ||
+      max_blocks <= 0 || !tiled_shape(head_dim, n_rep))
+    return 0;
+  const int n_groups = (num_q_heads + n_rep - 1) / n_rep;
+  const int64_t rows = (int64_t)total_q * num_q_heads;
+  const BlockPlan plan = plan_for(batch, rows, max_chunk, n_groups, head_dim, n_rep, max_blocks, true, quant);
+  if (plan.parts <= 1) return 0;
+  const size_t bytes = part_bytes(plan.parts, rows, head_dim);
+  return bytes > kMaxPartBytes ? 0 : bytes;
 }
 
 constexpr int kMergeWgs = 2048;

@@ -487,7 +487,7 @@ int prefill_impl(const void* q, const void* k_cache, const void* v_cache, const 
   }
   if (fast) {
     const bool fine = fine_shape(head_dim, n_rep);
-    const int64_t wgs = plan_launch(a, total_q, workspace, workspace_bytes);
+    const int64_t wgs = plan_launch(a, total_q, false, workspace, workspace_bytes);
     // The 64-dim instances write no statistics: every row is flagged, and the scoring pass recomputes
     // them from the keys.
     const int obs_rows = obs && head_dim == 64 ? a.obs : 0;
@@ -560,15 +560,7 @@ extern "C" int ukv_paged_prefill_obs_stats(const void* q, const void* k_cache, c
 
 extern "C" size_t ukv_paged_prefill_workspace_bytes(int batch, int total_q, int max_chunk, int num_q_heads,
                                                     int num_kv_heads, int head_dim, int n_rep, int max_blocks) {
-  if (batch <= 0 || total_q <= 0 || max_chunk <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || n_rep < 1 ||
-      max_blocks <= 0 || !tiled_shape(head_dim, n_rep))
-    return 0;
-  const int n_groups = (num_q_heads + n_rep - 1) / n_rep;
-  const int64_t rows = (int64_t)total_q * num_q_heads;
-  const BlockPlan plan = plan_for(batch, rows, max_chunk, n_groups, head_dim, n_rep, max_blocks, true);
-  if (plan.parts <= 1) return 0;
-  const size_t bytes = part_bytes(plan.parts, rows, head_dim);
-  return bytes > kMaxPartBytes ? 0 : bytes;
+  return parts_workspace(batch, total_q, max_chunk, num_q_heads, num_kv_heads, head_dim, n_rep, max_blocks, false);
 }
 
 extern "C" int ukv_paged_prefill_parts(const void* q, const void* k_cache, const void* v_cache,

@@ -534,6 +534,5 @@ extern "C" size_t ukv_quant_prefill_workspace_bytes(int batch, int total_q, int 
       max_blocks <= 0)
     return 0;
   return std::max(quant_chunk_workspace(batch, num_q_heads, n_rep, head_dim, max_chunk, max_blocks),
-                  ukv_paged_prefill_workspace_bytes(batch, total_q, max_chunk, num_q_heads, num_kv_heads, head_dim,
-                                                    n_rep, max_blocks));
+                  quant_parts_workspace(batch, total_q, max_chunk, num_q_heads, num_kv_heads, head_dim, n_rep, max_blocks));
 }

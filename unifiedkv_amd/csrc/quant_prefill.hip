@@ -20,6 +20,11 @@ template <int DT> void launch_quant(const QuantPrefillArgs& a, int format, bool 
 
 }  // namespace
 
+size_t quant_parts_workspace(int batch, int total_q, int max_chunk, int num_q_heads, int num_kv_heads, int head_dim,
+                             int n_rep, int max_blocks) {
+  return parts_workspace(batch, total_q, max_chunk, num_q_heads, num_kv_heads, head_dim, n_rep, max_blocks, true);
+}
+
 // (arguments checked by the caller)
 int quant_prefill(const QuantAttnArgs& x, int total_q, int dtype, int format, void* workspace, size_t workspace_bytes,
                   hipStream_t stream) {
@@ -74,7 +79,7 @@ int quant_prefill(const QuantAttnArgs& x, int total_q, int dtype, int format, vo
   a.scale = x.scale;
   a.scale_log2 = x.scale * kLog2e;
   const bool fine = fine_shape(x.D, x.n_rep);
-  const int64_t wgs = plan_launch(a, total_q, workspace, workspace_bytes);
+  const int64_t wgs = plan_launch(a, total_q, true, workspace, workspace_bytes);
   if (wgs > INT32_MAX) return UKV_ERR_INVALID_ARGUMENT;
   if (wgs > 0)
     dtype == UKV_DTYPE_BF16 ? launch_quant<UKV_DTYPE_BF16>(a, format, fine, (unsigned)wgs, stream)

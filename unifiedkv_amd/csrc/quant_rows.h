@@ -22,9 +22,12 @@ struct QuantAttnArgs {
 int quant_decode(const QuantAttnArgs& a, int dtype, int format, void* workspace, size_t workspace_bytes,
                  hipStream_t stream);
 
-// quant_prefill.hip; the workspace (null: none) is ukv_paged_prefill_workspace_bytes().
+// quant_prefill.hip; the workspace (null: none) is of quant_parts_workspace() bytes.
 int quant_prefill(const QuantAttnArgs& a, int total_q, int dtype, int format, void* workspace, size_t workspace_bytes,
                   hipStream_t stream);
+
+size_t quant_parts_workspace(int batch, int total_q, int max_chunk, int num_q_heads, int num_kv_heads, int head_dim,
+                             int n_rep, int max_blocks);
 
 // quant_split.hip: chunks of a few queries. Returns whether the split kernel takes them (with this workspace, of
 // quant_chunk_workspace() bytes), and then the status.
