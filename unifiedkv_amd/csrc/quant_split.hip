@@ -18,10 +18,6 @@
 // codes, and within 10 % of it for int8 (five for four).
 #include <type_traits>
 
-#ifndef UKV_QUANT_SETS
-#define UKV_QUANT_SETS 2
-#endif
-
 #include "page16_split.h"
 #include "quant_common.h"
 #include "quant_rows.h"
@@ -88,9 +84,6 @@ __device__ __forceinline__ void v_operands(const P& pg, int c, const f16x2 (&sca
 template <int DT, int D, int CB, bool CHUNK, int MODE, int QF>
 __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(const QuantSplitArgs a) {
   constexpr int DPL = D / 16, STEPS = D / 32, KJ = D / 64, VW = D / 64;
-  // Register sets of a page: kAhead pages are in flight while one is reduced. A window of page ids, a lane each, is
-  // whole rounds of the sets.
-  constexpr int kSets = D > 128 ? 1 : UKV_QUANT_SETS, kAhead = D > 128 ? 1 : kSets - 1, kWindow = 64 / kSets * kSets;
   constexpr float kTau = 8.f;
   constexpr bool SHARED = MODE != kSplit, DIRECT = MODE == kDirect;
   static_assert(CHUNK || CB == 1, "one query's heads are one column block");
@@ -203,8 +196,8 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
     return s;
   };
   auto page_at = [&](const Segment& s, int i) -> int { return SHARED ? s.pa + sub + i * subs : s.pa + i; };
-  auto window_ids = [&](const Segment& s, int i0) -> int {  // ids of the wave's pages i0 + lane, a window of them
-    return lane < kWindow && i0 + lane < s.n_mine ? a.bt[(int64_t)s.b * a.max_blocks + page_at(s, i0 + lane)] : 0;
+  auto window_ids = [&](const Segment& s, int i0) -> int {  // ids of the wave's pages i0 + lane
+    return i0 + lane < s.n_mine ? a.bt[(int64_t)s.b * a.max_blocks + page_at(s, i0 + lane)] : 0;
   };
 
   u32x4 qb[CB][STEPS];  // B operands of the scores: column i16 of each block (zero where there is none)
@@ -380,8 +373,8 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
     }
   };
 
-  CodePage<D> sets[kSets];
-  bool primed = false;  // the sets hold the segment's first pages, loaded at the end of the one before
+  CodePage<D> page;
+  bool primed = false;  // it is the segment's first page, loaded at the end of the one before
   Segment s = segment(b_first, x0 - s_first, x1 - x0);
   int x = x0;  // global index of the segment's first page
   int bid_win = window_ids(s, 0);
@@ -400,7 +393,7 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
       nx = segment(b, 0, x1 - x);
       bid_after = window_ids(nx, 0);
     }
-    int bid_next = window_ids(s, kWindow), w_begin = 0;
+    int bid_next = window_ids(s, 64), w_begin = 0;
 
     int q0 = s.b, C = 1;  // the sequence's first query row, and its queries
     if constexpr (CHUNK) {
@@ -433,27 +426,24 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
     }
 
     if (s.n_mine > 0) {
-      // Page i of the wave, into a set. Past its last page: that one again (a load of known age, which the compiler's
-      // waits count), or, where the next segment starts in this set, its page `after`.
-      auto load = [&](CodePage<D>& pg, int i, int after) {
+      // Page i of the wave; past its last page the next segment's first, or, where there is none, the last again (a load
+      // of known age, which the compiler's waits count).
+      auto load = [&](CodePage<D>& pg, int i) {
         int bid, key0, L = s.L;
-        if (after >= 0 && i >= s.n_mine && nx.n_mine > 0) {
-          after = min(after, nx.n_mine - 1);
-          bid = __builtin_amdgcn_readlane(bid_after, after);
-          key0 = 16 * page_at(nx, after);
+        if (i >= s.n_mine && nx.n_mine > 0) {
+          bid = __builtin_amdgcn_readlane(bid_after, 0);
+          key0 = 16 * page_at(nx, 0);
           L = nx.L;
         } else {
           i = min(i, s.n_mine - 1);
           const int l = i - w_begin;
           bid = __builtin_amdgcn_readlane(bid_win, l & 63);
-          if (l >= kWindow) bid = __builtin_amdgcn_readlane(bid_next, l - kWindow);
+          if (l >= 64) bid = __builtin_amdgcn_readlane(bid_next, l - 64);
           key0 = 16 * page_at(s, i);
         }
         load_page(pg, bid, key0, L);
       };
-      if (!primed)
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) load(sets[u], u, -1);
+      if (!primed) load(page, 0);
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
         q_scale[cb] = a.scale_log2;
@@ -463,23 +453,29 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
           q_scale[cb] *= query_scale(top);
         }
       }
+      // One copy of the loop's body, the page in flight handed on by register moves: 19 of them against a body that the
+      // instruction cache holds sooner and that leaves HBM more even (two copies in turn took 16.4 us against 14.8 for four
+      // sequences of 256-2048 tokens, 90 against 86.5 for 64 ragged ones and 176 against 172 for 16 x 32K; at 64 dims, whose
+      // pages are short, 117 against 113 for the last, but 57 against 62 for the ragged ones. More pages in flight only
+      // lost).
       while (true) {
-        const int end = min(s.n_mine, w_begin + kWindow);
-        for (int i = w_begin; i < end; i += kSets)
-#pragma unroll
-          for (int u = 0; u < kSets; ++u) {
-            if constexpr (kSets == 1) {
-              process(sets[0]);
-              load(sets[0], i + 1, 0);
-            } else {
-              load(sets[(u + kAhead) % kSets], i + u + kAhead, u - 1);
-              if (u == 0 || i + u < s.n_mine) process(sets[u]);
-            }
+        const int end = min(s.n_mine, w_begin + 64);
+#pragma unroll 1
+        for (int i = w_begin; i < end; ++i) {
+          if constexpr (D > 128) {  // (no registers for a second page)
+            process(page);
+            load(page, i + 1);
+          } else {
+            CodePage<D> ahead;
+            load(ahead, i + 1);
+            process(page);
+            page = ahead;
           }
-        w_begin += kWindow;
+        }
+        w_begin += 64;
         if (w_begin >= s.n_mine) break;
         bid_win = bid_next;
-        bid_next = window_ids(s, w_begin + kWindow);
+        bid_next = window_ids(s, w_begin + 64);
       }
     }
     primed = s.n_mine > 0 && nx.n_mine > 0;
