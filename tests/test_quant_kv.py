@@ -142,6 +142,9 @@ def test_c_entry_points_refuse_bad_arguments():
         assert write(**bad) == _ext.UKV_ERR_INVALID_ARGUMENT
     assert lib.ukv_quant_prefill(16, 16, 16, 16, 16, s, 1, 16, None, 16, 16, 1, 4, 4, 4, 1, 64, 4, 1, q2, 0.1, 0, 0, None,
                                  0, None) == _ext.UKV_ERR_INVALID_ARGUMENT
+    for i in range(8):  # nothing to attend: no scratch
+        assert lib.ukv_quant_prefill_workspace_bytes(*[0 if j == i else 4 for j in range(8)]) == 0 or i == 5
+    assert lib.ukv_quant_prefill_workspace_bytes(4, 8, 2, 8, 2, 64, 4, 4) > 0
 
 
 def test_pool_refusals():
@@ -306,6 +309,34 @@ def test_append_equals_a_chunk_of_one_and_skips_bad_pages(cuda, fmt):
         np.testing.assert_array_equal(x, y)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("H, D", [(1, 32), (1, 64), (3, 32), (1, 128), (8, 128)])
+def test_whole_pages_outside_the_pool_are_left_alone(cuda, fmt, H, D):
+    """Pages whose sixteen tokens are all written, with ids below and above the pool's, between good ones."""
+    rng = np.random.default_rng(H * D)
+    N, n = 12, 16 * 7 + 3
+    table = np.array([[3, -1, 5, N, 11, 1 << 30, 0, 7]], dtype=np.int32)
+    layer = _layer(cuda, fmt, N, H, D)
+    before = _bits(layer)
+    rows = [torch.from_numpy(rng.standard_normal((n, H, D))).half() for _ in range(2)]
+    quant_kv.write_chunk_kv(layer, rows[0].to(cuda), rows[1].to(cuda), _dev(table, cuda), [0, n], [n])
+    good = [(i, p) for i, p in enumerate(table[0]) if 0 <= p < N]
+    rest = [p for p in range(N) if p not in table[0]]
+    for x, y, e in zip(rows, _values(layer, fmt), _bits(layer)[2:]):
+        want, exps = qo.quantise(x.double().numpy(), fmt)
+        for i, p in good:
+            m = min(16, n - 16 * i)
+            np.testing.assert_array_equal(y[p, :m], want[16 * i:16 * i + m])
+            np.testing.assert_array_equal(e[p].transpose(2, 0, 1)[:m], exps[16 * i:16 * i + m])
+    for x, y in zip(before, _bits(layer)):
+        np.testing.assert_array_equal(x[rest], y[rest])
+    back = quant_kv.read_kv(layer, _dev(table, cuda), [0, n], [n], dtype=torch.float16)
+    for r in back:
+        for i in (1, 3, 5):
+            assert not r[16 * i:16 * i + 16].any()
+
+
 def _bound(out, spread, v, q, k, scale, dtype, weight):
     """How far a result may be off: half a step of its type, then what the weights may be off by, in units of
     sum(p |v|) and once more for their sum. A weight is off by its own rounding (``weight``, relative), by the
@@ -450,6 +481,81 @@ def test_long_chunks_match_the_oracle(cuda, fmt, pre, chunk, H, n_rep, D):
         spans = [(cu[b] + i, b, pre[b] + i + 1) for b in range(len(pre))
                  for i in sorted({0, chunk[b] - 1, chunk[b] // 2, chunk[b] // 3})]
         _check_rows(got, layer, fmt, q, table, spans, 0.1, n_rep, CHUNK_WEIGHT, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("batch, most, lo, hi, H, n_rep, D", [
+    (70, 4, 1, 700, 2, 4, 128), (70, 8, 1, 700, 6, 4, 128), (66, 3, 1, 300, 3, 5, 64), (3, 2, 100, 900, 12, 8, 64),
+    (40, 5, 300, 600, 9, 6, 64), (2, 1, 1, 5000, 2, 16, 128), (5, 3, 60000, 65000, 5, 4, 64),
+    (4, 7, 66000, 70000, 6, 4, 128)])
+def test_few_queries_a_sequence_over_ragged_lengths(cuda, fmt, batch, most, lo, hi, H, n_rep, D):
+    """Drafted tokens: chunks of none to ``most`` queries, more sequences than a wave has lanes, more KV heads than a
+    workgroup has waves, more pages a wave than its lanes hold ids of. Sequences share pages."""
+    rng = np.random.default_rng(batch + H)
+    N = 300
+    layer = _filled(cuda, fmt, torch.bfloat16, rng, N, H, D)
+    lens = [int(x) for x in rng.integers(lo, hi, size=batch, endpoint=True)]
+    chunk = [min(n, int(c)) for n, c in zip(lens, rng.integers(0, most, size=batch, endpoint=True))]
+    chunk[-1] = min(lens[-1], most)
+    table = rng.integers(0, N, size=(batch, -(-max(lens) // 16) + 2)).astype(np.int32)
+    table[batch // 2, 0] = N  # sixteen keys without a page
+    cu = np.concatenate([[0], np.cumsum(chunk)])
+    some = sorted({0, 1, batch // 2, batch - 1} | {int(x) for x in rng.integers(0, batch, 3)})
+    spans = [(cu[b] + i, b, lens[b] - chunk[b] + i + 1) for b in some for i in sorted({0, chunk[b] - 1}) if 0 <= i < chunk[b]]
+    for dt in DTYPES.values():
+        q = torch.from_numpy(rng.standard_normal((sum(chunk), H * n_rep, D))).to(dt).to(cuda)
+        got = quant_kv.prefill_attention(q, layer, _dev(table, cuda), _dev(cu, cuda), _dev(lens, cuda), softmax_scale=0.1,
+                                         n_rep=n_rep, max_chunk=most)
+        _check_rows(got, layer, fmt, q, table, spans, 0.1, n_rep, CHUNK_WEIGHT, N)
+    dq = torch.from_numpy(rng.standard_normal((batch, H * n_rep, D))).half().to(cuda)
+    got = quant_kv.decode_attention(dq, layer, _dev(table, cuda), _dev(lens, cuda), softmax_scale=0.1, n_rep=n_rep)
+    _check_rows(got, layer, fmt, dq, table, [(b, b, lens[b]) for b in some], 0.1, n_rep, DECODE_WEIGHT, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("most, H, n_rep, D", [(3, 2, 4, 128), (8, 2, 4, 128), (4, 8, 4, 64), (6, 5, 4, 64)])
+def test_nan_blocks_among_few_queries(cuda, fmt, most, H, n_rep, D):
+    """A NaN block at every place of the chunk and right before it: only the queries that see it turn NaN, in the
+    value's block's dims alone, and every one where a key holds it."""
+    rng = np.random.default_rng(most)
+    batch = 16
+    layer = _filled(cuda, fmt, torch.float16, rng, 40 * batch, H, D)
+    lens, chunk = [500 + 3 * b for b in range(batch)], [most] * batch
+    table = _tables(rng, 40 * batch, lens, extra=64 - 35)  # (a table wide enough for two column blocks)
+    bad = torch.ones((1, H, D), dtype=torch.float16, device=cuda)
+    bad[:, :, 32:64] = float("inf")
+    for b in range(batch):
+        pos = lens[b] - most + b // 2 - 1
+        if pos < lens[b]:
+            rows = (bad, torch.ones_like(bad)) if b % 2 else (torch.ones_like(bad), bad)
+            quant_kv.write_chunk_kv(layer, *rows, _dev(table[b:b + 1], cuda), [0, 1], [pos + 1])
+    cu = np.arange(batch + 1) * most
+    q = torch.from_numpy(rng.standard_normal((batch * most, H * n_rep, D))).half().to(cuda)
+    got = quant_kv.prefill_attention(q, layer, _dev(table, cuda), _dev(cu, cuda), _dev(lens, cuda), softmax_scale=0.1,
+                                     n_rep=n_rep, max_chunk=most)
+    spans = [(cu[b] + i, b, lens[b] - most + i + 1) for b in range(batch) for i in range(most)]
+    _check_rows(got, layer, fmt, q, table, spans, 0.1, n_rep, CHUNK_WEIGHT, 40 * batch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_chunks_without_scratch(cuda, fmt, monkeypatch):
+    """No workspace: one kernel over whole keys, for few queries and for many."""
+    from unifiedkv_amd import _ext
+
+    rng = np.random.default_rng(12)
+    H, R, D, N, lens = 2, 4, 128, 300, [2000, 900, 40]
+    layer = _filled(cuda, fmt, torch.float16, rng, N, H, D)
+    table = _tables(rng, N, lens)
+    monkeypatch.setattr(_ext.load(), "ukv_quant_prefill_workspace_bytes", lambda *a: 0)
+    for chunk in ([3, 1, 4], [200, 90, 40]):
+        cu = np.concatenate([[0], np.cumsum(chunk)])
+        q = torch.from_numpy(rng.standard_normal((sum(chunk), H * R, D))).half().to(cuda)
+        got = quant_kv.prefill_attention(q, layer, _dev(table, cuda), list(cu), lens, softmax_scale=0.1, n_rep=R)
+        spans = [(cu[b] + i, b, lens[b] - c + i + 1) for b, c in enumerate(chunk) for i in sorted({0, c // 2, c - 1})]
+        _check_rows(got, layer, fmt, q, table, spans, 0.1, R, CHUNK_WEIGHT, N)
 
 
 @pytest.mark.gpu

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantRowsArgs a)
         }
       }
     }
-    if (!together) return;
+    if (!together || page < 0) return;  // (a small page's other threads have not met its id yet)
     __syncthreads();
     for (int y = threadIdx.x; y < 2 * blocks; y += 256) {
       const bool is_v = y >= blocks;
