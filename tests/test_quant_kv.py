@@ -132,13 +132,16 @@ def test_c_entry_points_refuse_bad_arguments():
     assert decode(q=None) == _ext.UKV_ERR_INVALID_ARGUMENT
     assert decode(blocks=-1) == _ext.UKV_ERR_INVALID_ARGUMENT
     assert decode(blocks=1 << 28) == _ext.UKV_ERR_INVALID_ARGUMENT
+    s16 = _ext.i64_array([1024] * 12)
+    assert lib.ukv_quant_decode(16, 16, 16, 16, 16, s16, 1, 16, 16, 16, 65536, 4, 1, 64, 4, 1, _ext.i64_array([256, 64]),
+                                0.1, 0, 0, None, 0, None) == _ext.UKV_ERR_INVALID_ARGUMENT
 
-    def write(fmt=0, dtype=0, heads=1, table=16, rows=16):
-        return lib.ukv_quant_kv_write(16, 16, 16, 16, s, 1, rows, rows, r4, table, 1, None, None, 0, 1, 1, heads, 64, fmt,
-                                      dtype, None)
+    def write(fmt=0, dtype=0, heads=1, table=16, rows=16, batch=1, chunk=1):
+        return lib.ukv_quant_kv_write(16, 16, 16, 16, s, 1, rows, rows, r4, table, 1, None, None, 0, batch, chunk, heads,
+                                      64, fmt, dtype, None)
 
     assert write(fmt=7) == _ext.UKV_ERR_DTYPE and write(dtype=3) == _ext.UKV_ERR_DTYPE
-    for bad in (dict(heads=0), dict(table=None), dict(rows=None)):
+    for bad in (dict(heads=0), dict(table=None), dict(rows=None), dict(batch=65536), dict(batch=1 << 15, chunk=1 << 16)):
         assert write(**bad) == _ext.UKV_ERR_INVALID_ARGUMENT
     assert lib.ukv_quant_prefill(16, 16, 16, 16, 16, s, 1, 16, None, 16, 16, 1, 4, 4, 4, 1, 64, 4, 1, q2, 0.1, 0, 0, None,
                                  0, None) == _ext.UKV_ERR_INVALID_ARGUMENT
@@ -720,6 +723,31 @@ def test_streams_and_captured_calls(cuda, fmt):
         for _, out in graphs:
             for a, b in zip(eager, out):
                 assert torch.equal(a, b), i
+
+
+@pytest.mark.gpu
+def test_another_current_device(cuda, monkeypatch):
+    """A launch goes to the current device: the layer's is made that one for the call."""
+    layer = _filled(cuda, "int8", torch.float16, np.random.default_rng(1), 8, 2, 64)
+    q, table, lens = torch.ones((1, 4, 64), dtype=torch.float16, device=cuda), _dev([[1, 2]], cuda), _dev([20], cuda)
+    calls = [lambda: quant_kv.decode_attention(q, layer, table, lens, softmax_scale=0.1, n_rep=2),
+             lambda: quant_kv.prefill_attention(q, layer, table, [0, 1], lens, softmax_scale=0.1, n_rep=2),
+             lambda: quant_kv.read_kv(layer, table, [0, 1], lens, dtype=torch.float16)[0]]
+    want = [c() for c in calls]
+    entered = []
+
+    class Guard(torch.cuda.device):
+        def __init__(self, device):
+            entered.append(torch.device(device))
+            super().__init__(device)
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(quant_kv, "_device_now", lambda: 1 + (cuda.index or 0))
+    for call, w in zip(calls, want):
+        entered.clear()
+        assert torch.equal(call(), w) and entered[-1] == layer.device
+    quant_kv.append_kv(layer, q[:, :2], q[:, :2], table, lens)
+    assert len(entered) == 2
 
 
 @pytest.mark.gpu

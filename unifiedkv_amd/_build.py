@@ -165,8 +165,9 @@ def _drain(procs):
 
 
 def _is_remark_context(ln: str) -> bool:
-    """The source excerpt clang prints under each remark (a line number gutter and a caret line)."""
-    return bool(re.match(r"^\s*\d+ \|", ln) or re.match(r"^\s*\|\s*\^", ln))
+    """What clang prints with a remark: the file that a header's kernel came in by, the source excerpt (a line number
+    gutter and a caret line)."""
+    return bool(re.match(r"^In file included from ", ln) or re.match(r"^\s*\d+ \|", ln) or re.match(r"^\s*\|\s*\^", ln))
 
 
 def guarded_resource_usage(src: str, jobs_flags=()) -> Dict[str, Dict[str, str]]:

@@ -64,7 +64,8 @@ template <int QF> __device__ __forceinline__ uint32_t quant_codes4(const float (
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(y[i] + 12582912.f);
-    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u);
+    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u);
     return lo | (hi << 16);
   } else {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);

@@ -95,7 +95,8 @@ __device__ __forceinline__ int div_small(int x, float inv) { return (int)(((floa
 
 // Rows of whole blocks (D a multiple of 32), 16-byte aligned: a workgroup takes a page, a thread eight dims of a (row,
 // head) at a time, K and V, kAtOnce loads of both before the first is used. A page's exponents, sixteen tokens
-// together, meet in LDS and go out as 16-byte stores; a part of a page's go out as bytes. Bound: HBM (reads two bytes, writes one).
+// together, meet in LDS and go out as 16-byte stores; a part of a page's go out as bytes. Bound: HBM (reads two bytes an
+// element, writes one): @@
 template <int DT, int QF>
 __global__ void __launch_bounds__(256) quant_write_kernel(const QuantRowsArgs a) {
   constexpr int kAtOnce = 4;
@@ -364,8 +365,8 @@ bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p)
 bool wide_rows(const QuantRowsArgs& a) {
   const int64_t rows = a.rk_st | a.rk_sh | a.rv_st | a.rv_sh;
   const int64_t codes = a.c.k_sp | a.c.k_st | a.c.k_sh | a.c.v_sp | a.c.v_st | a.c.v_sh;
-  return a.D % kQuantBlock == 0 && a.H * a.D <= 32768 && ((rows | codes) & 7) == 0 && aligned(a.rows_k, 16) && aligned(a.rows_v, 16) &&
-         aligned(a.c.k, 8) && aligned(a.c.v, 8);
+  return a.D % kQuantBlock == 0 && (int64_t)a.H * a.D <= 32768 && ((rows | codes) & 7) == 0 && aligned(a.rows_k, 16) &&
+         aligned(a.rows_v, 16) && aligned(a.c.k, 8) && aligned(a.c.v, 8);
 }
 
 constexpr int kSlice = 64;
@@ -404,6 +405,7 @@ int rows_call(bool write, const void* k, const void* v, const void* ks, const vo
   if (batch < 0 || max_chunk < 0 || num_heads <= 0 || head_dim <= 0 || max_blocks < 0 || num_pages < 0)
     return UKV_ERR_INVALID_ARGUMENT;
   if (batch > 65535 || max_blocks > (INT32_MAX >> 4)) return UKV_ERR_INVALID_ARGUMENT;
+  if (!cu_seqlens && (int64_t)batch * max_chunk > INT32_MAX) return UKV_ERR_INVALID_ARGUMENT;  // (rows are numbered in ints)
   if (batch == 0 || max_chunk == 0) return UKV_OK;
   if (!k || !v || !ks || !vs || !layer_strides || !rows_k || !rows_v || !row_strides) return UKV_ERR_INVALID_ARGUMENT;
   if (max_blocks > 0 && !block_table) return UKV_ERR_INVALID_ARGUMENT;

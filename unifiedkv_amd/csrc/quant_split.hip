@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       const bool live = col_live(cb, i16);
-      const uint16_t* qp = a.q + (live ? (int64_t)(q0 + col_query(cb, i16)) * a.q_sb + (int64_t)col_head(cb, i16) * a.q_sh : 0);
+      const uint16_t* qp =
+          a.q + (live ? (int64_t)(q0 + col_query(cb, i16)) * a.q_sb + (int64_t)col_head(cb, i16) * a.q_sh : 0);
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
@@ -453,11 +454,11 @@ __global__ void __launch_bounds__(64 * UKV_PAGE16_WAVES, 1) quant_split_kernel(c
           q_scale[cb] *= query_scale(top);
         }
       }
-      // One copy of the loop's body, the page in flight handed on by register moves: 19 of them against a body that the
-      // instruction cache holds sooner and that leaves HBM more even (two copies in turn took 16.4 us against 14.8 for four
-      // sequences of 256-2048 tokens, 90 against 86.5 for 64 ragged ones and 176 against 172 for 16 x 32K; at 64 dims, whose
-      // pages are short, 117 against 113 for the last, but 57 against 62 for the ragged ones. More pages in flight only
-      // lost).
+      // One copy of the loop's body, the page in flight handed on by register moves: 19 of them against a body that
+      // the instruction cache holds sooner and that leaves HBM more even (two copies in turn took 16.4 us against 14.8
+      // for four sequences of 256-2048 tokens, 90 against 86.5 for 64 ragged ones and 176 against 172 for 16 x 32K; at
+      // 64 dims, whose pages are short, 117 against 113 for the last, but 57 against 62 for the ragged ones. More pages
+      // in flight only lost).
       while (true) {
         const int end = min(s.n_mine, w_begin + 64);
 #pragma unroll 1
@@ -552,7 +553,8 @@ template <int DT, int D> __global__ void __launch_bounds__(256) quant_chunk_comb
       for (int d = threadIdx.x; d < D; d += 256) a.out[((int64_t)(q0 + i) * a.Hq + h) * D + d] = 0x7FFFu;
     return;
   }
-  combine_row<DT, D>(a, b, (int64_t)a.max_chunk * a.Hq, (int64_t)qi * a.Hq + h, a.out + ((int64_t)(q0 + qi) * a.Hq + h) * D);
+  combine_row<DT, D>(a, b, (int64_t)a.max_chunk * a.Hq, (int64_t)qi * a.Hq + h,
+                     a.out + ((int64_t)(q0 + qi) * a.Hq + h) * D);
 }
 
 namespace {
@@ -694,13 +696,15 @@ int quant_decode(const QuantAttnArgs& x, int dtype, int format, void* workspace,
                  hipStream_t stream) {
   if (!((x.D == 64 || x.D == 128 || x.D == 256) && x.n_rep <= 16 && split_layout(x)))
     return quant_rows_attention(x, x.B, dtype, format, stream);
+  if (x.B > 65535) return UKV_ERR_INVALID_ARGUMENT;  // (the merge's grid)
   const WorkspaceLayout w = workspace_layout(x.B, x.Hq, x.D, x.max_blocks);
   if (!workspace || workspace_bytes < w.total || !aligned16(workspace)) return UKV_ERR_WORKSPACE;
   return launch(x, false, w, dtype, format, workspace, stream);
 }
 
 size_t quant_chunk_workspace(int batch, int hq, int n_rep, int d, int max_chunk, int max_blocks) {
-  return chunk_shape(batch, max_chunk, n_rep, d, max_blocks) ? chunk_layout(batch, hq, d, max_chunk, max_blocks).total : 0;
+  if (!chunk_shape(batch, max_chunk, n_rep, d, max_blocks)) return 0;
+  return chunk_layout(batch, hq, d, max_chunk, max_blocks).total;
 }
 
 bool quant_chunk(const QuantAttnArgs& x, int dtype, int format, void* workspace, size_t workspace_bytes,

@@ -93,7 +93,16 @@ def _check_device(layer: QuantLayer, *tensors: torch.Tensor) -> None:
             raise RuntimeError("quant_kv_unavailable:device")
 
 
-def _check(code: int, layer: QuantLayer) -> None:
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(entry, layer: QuantLayer, *args) -> None:
+    """A C entry's call with the layer's device as the current one, which is where it launches."""
+    if layer.device.index == _device_now():
+        code = entry(*args)
+    else:
+        with torch.cuda.device(layer.device):
+            code = entry(*args)
     if code != _ext.UKV_OK:
         if code == _ext.UKV_ERR_HEAD_DIM:
             _refuse(f"head_dim_{layer.head_dim}")
@@ -108,19 +117,21 @@ def _batch(cu, lens, table) -> int:
 
 
 def _write(layer, k, v, bt, cu, lens, lens_add, batch, max_chunk) -> None:
-    _check(_ext.load().ukv_quant_kv_write(
+    _launch(
+        _ext.load().ukv_quant_kv_write, layer,
         *layer.pointers, layer.strides, layer.num_pages, k.data_ptr(), v.data_ptr(),
         _ext.i64_tuple(k.stride()[:2] + v.stride()[:2]), bt.data_ptr(), int(bt.shape[1]),
         None if cu is None else cu.data_ptr(), None if lens is None else lens.data_ptr(), lens_add, batch, max_chunk,
-        layer.num_heads, layer.head_dim, layer.format_code, _DTYPE_CODES[k.dtype], _current_stream(layer.device)), layer)
+        layer.num_heads, layer.head_dim, layer.format_code, _DTYPE_CODES[k.dtype], _current_stream(layer.device))
 
 
 def _read(layer, k, v, bt, cu, lens, batch, max_chunk) -> None:
-    _check(_ext.load().ukv_quant_kv_read(
+    _launch(
+        _ext.load().ukv_quant_kv_read, layer,
         *layer.pointers, layer.strides, layer.num_pages, k.data_ptr(), v.data_ptr(),
         _ext.i64_tuple(k.stride()[:2] + v.stride()[:2]), bt.data_ptr(), int(bt.shape[1]),
         None if cu is None else cu.data_ptr(), None if lens is None else lens.data_ptr(), batch, max_chunk,
-        layer.num_heads, layer.head_dim, layer.format_code, _DTYPE_CODES[k.dtype], _current_stream(layer.device)), layer)
+        layer.num_heads, layer.head_dim, layer.format_code, _DTYPE_CODES[k.dtype], _current_stream(layer.device))
 
 
 def write_chunk_kv(layer: QuantLayer, k_new: torch.Tensor, v_new: torch.Tensor, block_table: torch.Tensor,
@@ -220,10 +231,11 @@ def decode_attention(q: torch.Tensor, layer: QuantLayer, block_table: torch.Tens
     stream = _current_stream(dev)
     width = int(bt.shape[1])
     ws = _workspace(B, Hq, D, width, dev, stream)
-    _check(_ext.load().ukv_quant_decode(
+    _launch(
+        _ext.load().ukv_quant_decode, layer,
         q.data_ptr(), *layer.pointers, layer.strides, layer.num_pages, bt.data_ptr(), lens.data_ptr(), out.data_ptr(),
         B, Hq, layer.num_heads, D, int(n_rep), width, _ext.i64_tuple(q.stride()[:2]), float(softmax_scale),
-        layer.format_code, _DTYPE_CODES[q.dtype], ws.data_ptr(), ws.numel(), stream), layer)
+        layer.format_code, _DTYPE_CODES[q.dtype], ws.data_ptr(), ws.numel(), stream)
     return out
 
 
@@ -260,11 +272,12 @@ def prefill_attention(q: torch.Tensor, layer: QuantLayer, block_table: torch.Ten
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
         except torch.OutOfMemoryError:  # without scratch the keys stay in one part
             need = 0
-    _check(lib.ukv_quant_prefill(
+    _launch(
+        lib.ukv_quant_prefill, layer,
         q.data_ptr(), *layer.pointers, layer.strides, layer.num_pages, bt.data_ptr(), cu.data_ptr(), lens.data_ptr(),
         out.data_ptr(), B, total_q, mc, Hq, layer.num_heads, D, int(n_rep), width, _ext.i64_tuple(q.stride()[:2]),
         float(softmax_scale), layer.format_code, _DTYPE_CODES[q.dtype], ws.data_ptr() if ws is not None else None,
-        need, _current_stream(dev)), layer)
+        need, _current_stream(dev))
     return out
 
 
@@ -360,7 +373,8 @@ class QuantizedKVPool(PagedKVPool):
         append_kv(self.layer(layer_id), self._as_pool_rows(k_tok.squeeze(1))[None],
                   self._as_pool_rows(v_tok.squeeze(1))[None], at[:1], at[1])
 
-    def read_kv_from_blocks(self, layer_id: int, block_ids: List[int], seq_len: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    def read_kv_from_blocks(self, layer_id: int, block_ids: List[int], seq_len: int
+                            ) -> Tuple[torch.Tensor, torch.Tensor]:
         """[h_kv, min(seq_len, 16 * len(block_ids)), d] K and V (core/pool.py:154-172)."""
         n = max(0, min(int(seq_len), 16 * len(block_ids)))
         if n == 0:
