@@ -502,8 +502,9 @@ int ukv_quant_decode(const void* q, const void* k, const void* v, const void* k_
 
 /*
  * ukv_paged_prefill_parts over the 8-bit cache, without statistics: packed chunk queries, causal, bottom right
- * aligned. The workspace (ukv_quant_prefill_workspace_bytes; may be NULL) lets a launch of few queries share its keys
- * among workgroups; without it each query block takes its keys alone, which a few queries behind long prefixes feel.
+ * aligned. The workspace (ukv_quant_prefill_workspace_bytes; may be NULL) lets workgroups share the keys, evenly by the
+ * lengths on the device where the call is long; without it each query block takes its keys alone, which a few queries
+ * behind long prefixes and sequences of different lengths feel. It needs no initialisation.
  * Replaces core/engine.py:1826-1854 for this cache.
  */
 size_t ukv_quant_prefill_workspace_bytes(int batch, int total_q, int max_chunk, int num_q_heads, int num_kv_heads,

@@ -542,6 +542,103 @@ def test_nan_blocks_among_few_queries(cuda, fmt, most, H, n_rep, D):
     _check_rows(got, layer, fmt, q, table, spans, 0.1, n_rep, CHUNK_WEIGHT, 40 * batch)
 
 
+def _in_shares(batch, total, most, H, n_rep, D, width):
+    """Whether a call's keys are cut by its lengths on the device (its partials are of that size, whatever the call's)."""
+    from unifiedkv_amd import _ext
+
+    need = _ext.load().ukv_quant_prefill_workspace_bytes(batch, total, most, H * n_rep, H, D, n_rep, width)
+    slots = 256 * (2 if D == 64 else 1)
+    return any(2 * slots * 128 * cb * (4 * D + 8) <= need < 2 * slots * 128 * cb * (4 * D + 8) + 8192 for cb in (1, 2, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("pre, chunk, H, n_rep, D, width", [
+    ([9000, 300, 0, 4000, 17], [200, 150, 33, 1, 0], 2, 4, 128, 2600),
+    ([700, 12000, 0, 40], [1, 120, 120, 77], 2, 7, 128, 3500),
+    ([30000, 5, 0, 2000, 900], [256, 200, 256, 31, 0], 2, 4, 64, 3400),
+    ([60, 0, 14000, 1000, 333, 1], [90, 90, 17, 64, 2, 90], 3, 5, 64, 3800),
+    ([3000 + 400 * (i % 9) for i in range(40)], [1 + i % 10 for i in range(40)], 1, 16, 128, 2100),
+    ([150 * i for i in range(30)], [(7 * i) % 25 for i in range(30)], 4, 8, 64, 1200),
+    ([0, 3], [1, 2], 1, 4, 128, 3200),
+    ([0, 0, 0], [0, 0, 3], 1, 4, 128, 2200)])
+def test_chunks_in_shares(cuda, fmt, pre, chunk, H, n_rep, D, width):
+    """Tables wide enough that the lengths on the device cut the work: blocks in one piece and in many, sequences
+    without queries, queries without keys, fewer tiles than workgroups. Sequences share pages."""
+    rng = np.random.default_rng(sum(pre) + D)
+    N, batch = 250, len(pre)
+    most = max(chunk) if max(chunk) > 3 else 2000  # (declared longer than they are)
+    lens = [p + c for p, c in zip(pre, chunk)]
+    layer = _filled(cuda, fmt, torch.bfloat16, rng, N, H, D)
+    table = rng.integers(0, N, size=(batch, width)).astype(np.int32)
+    table[batch // 2, 1] = -5  # keys without a page
+    table[0, 3] = N
+    cu = np.concatenate([[0], np.cumsum(chunk)])
+    assert _in_shares(batch, sum(chunk), most, H, n_rep, D, width)
+    some = sorted({0, 1, min(2, batch - 1), batch - 1} | {int(x) for x in rng.integers(0, batch, 3)})
+    spans = [(cu[b] + i, b, lens[b] - chunk[b] + i + 1) for b in some
+             for i in sorted({0, chunk[b] // 3, chunk[b] // 2, chunk[b] - 1}) if 0 <= i < chunk[b]]
+    short = [max(0, n - c // 2 - 1) for n, c in zip(lens, chunk)]  # kv_lens below the chunk's: queries before key 0
+    for dt in DTYPES.values():
+        q = torch.from_numpy(rng.standard_normal((sum(chunk), H * n_rep, D))).to(dt).to(cuda)
+        got = quant_kv.prefill_attention(q, layer, _dev(table, cuda), _dev(cu, cuda), _dev(lens, cuda), softmax_scale=0.1,
+                                         n_rep=n_rep, max_chunk=most)
+        _check_rows(got, layer, fmt, q, table, spans, 0.1, n_rep, CHUNK_WEIGHT, N)
+        again = quant_kv.prefill_attention(q, layer, _dev(table, cuda), _dev(cu, cuda), _dev(lens, cuda),
+                                           softmax_scale=0.1, n_rep=n_rep, max_chunk=most)
+        assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+        if min(pre) == 0:
+            got = quant_kv.prefill_attention(q, layer, _dev(table, cuda), _dev(cu, cuda), _dev(short, cuda),
+                                             softmax_scale=0.1, n_rep=n_rep, max_chunk=most)
+            rows = [(r, b, max(0, n + short[b] - lens[b])) for r, b, n in spans]
+            _check_rows(got, layer, fmt, q, table, rows, 0.1, n_rep, CHUNK_WEIGHT, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n_rep, D, width", [(4, 128, 4200), (7, 128, 2200), (4, 64, 5600)])
+def test_shares_with_nan_blocks_and_a_chunk_longer_than_declared(cuda, fmt, n_rep, D, width):
+    rng = np.random.default_rng(D)
+    H, N, pre, chunk, most = 2, 300, [1500, 700, 4000, 90], [180, 200, 150, 160], 180
+    lens = [p + c for p, c in zip(pre, chunk)]
+    layer = _filled(cuda, fmt, torch.float16, rng, N, H, D)
+    table = np.zeros((4, width), dtype=np.int32)
+    table[:, :300] = rng.integers(0, 290, size=(4, 300))
+    table[0, lens[0] // 16], table[2, 60], table[3, 14] = 291, 292, 293  # pages of their own
+    bad = torch.ones((1, H, D), dtype=torch.float16, device=cuda)
+    bad[:, :, 32:] = float("nan")
+    one = torch.ones_like(bad)
+    for b, pos, rows in ((0, lens[0], (bad, bad)), (2, 960, (one, bad)), (3, 230, (bad, one))):
+        quant_kv.write_chunk_kv(layer, *rows, _dev(table[b:b + 1], cuda), [0, 1], [pos + 1])
+    cu = np.concatenate([[0], np.cumsum(chunk)])
+    q = torch.from_numpy(rng.standard_normal((sum(chunk) + 5, H * n_rep, D))).half().to(cuda)
+    assert _in_shares(4, sum(chunk) + 5, most, H, n_rep, D, width)
+    args = (layer, _dev(table, cuda), _dev(cu, cuda), _dev(lens, cuda))
+
+    def call():
+        return quant_kv.prefill_attention(q, *args, softmax_scale=0.1, n_rep=n_rep, max_chunk=most)
+
+    got = call()
+    assert torch.isnan(got[cu[1]:cu[2]]).all()  # longer than declared
+    spans = [(cu[b] + i, b, pre[b] + i + 1) for b in (0, 2, 3)
+             for i in sorted({0, 1, chunk[b] // 2, chunk[b] - 20, chunk[b] - 19, chunk[b] - 1})]
+    _check_rows(got, layer, fmt, q, table, spans, 0.1, n_rep, CHUNK_WEIGHT, N)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for _ in range(3):
+        q.mul_(-1)
+        for g, _ in graphs:
+            g.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[:cu[4]].view(torch.int16), eager[:cu[4]].view(torch.int16))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FMTS)
 def test_chunks_without_scratch(cuda, fmt, monkeypatch):

@@ -32,6 +32,7 @@ SOURCES = [
     "quant_kv.hip",
     "quant_split.hip",
     "quant_prefill.hip",
+    "quant_shares.hip",
 ]
 
 # Packed-FP32 VALU instructions are disabled for all device code.
@@ -55,6 +56,7 @@ SOURCE_FLAGS: Dict[str, List[str]] = {
     "paged_prefill.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "snapkv_score.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "quant_prefill.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    "quant_shares.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
 }
 
 
@@ -65,8 +67,9 @@ SOURCE_FLAGS: Dict[str, List[str]] = {
 # every instance must compile with ScratchSize 0 and no spilled VGPRs. (SGPRs spilled into the
 # lanes of a VGPR the compiler reserves for that purpose touch no load destination and no
 # memory; once no such lane is left they go through scratch, which ScratchSize reports.)
-GUARDED_SOURCES = ("page16_decode.hip", "paged_prefill.hip", "snapkv_score.hip", "quant_prefill.hip")
-GUARDED_KERNELS = ("page16_split_kernel", "paged_prefill_kernel", "snap_tile_kernel")
+GUARDED_SOURCES = ("page16_decode.hip", "paged_prefill.hip", "snapkv_score.hip", "quant_prefill.hip",
+                   "quant_shares.hip")
+GUARDED_KERNELS = ("page16_split_kernel", "paged_prefill_kernel", "snap_tile_kernel", "quant_shares_kernel")
 REMARK_FLAG = "-Rpass-analysis=kernel-resource-usage"
 
 _FN_RE = re.compile(r"remark: Function Name: (\S+)")

@@ -61,6 +61,8 @@ struct QuantPrefillArgs : PrefillArgs {
   const uint8_t* ks;
   const uint8_t* vs;
   int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
+  int share_blocks;    // shares (quant_prefill.hip): query blocks of a pair at most
+  int32_t* share_map;  // [B * share_blocks + 2]
 };
 template <int QF> struct TileArgs { typedef QuantPrefillArgs type; };
 template <> struct TileArgs<kCache16> { typedef PrefillArgs type; };
@@ -220,8 +222,8 @@ __device__ void prefill_cols_fp32(const PrefillArgs& a, int b, int g, int q_begi
 }
 
 // The same over the 8-bit cache, for a workgroup whose visible or masked values hold a NaN (zero weights make NaN of
-// it).
-template <int DT, int D, int QF>
+// it). SHARES: `part` is the slot of a piece (prefill_tile).
+template <int DT, int D, int QF, bool SHARES>
 __device__ void prefill_cols_fp32(const QuantPrefillArgs& a, int b, int g, int q_begin, int C, int P0, int Lk, int c0,
                                   int n_cols, int wv, int nwaves, int lane, int part, int key_a, int key_b) {
   constexpr int W = D / 64;  // dims per lane
@@ -263,7 +265,8 @@ __device__ void prefill_cols_fp32(const QuantPrefillArgs& a, int b, int g, int q
       m = mn;
     }
     if (part >= 0) {
-      const int64_t row = ((int64_t)part * a.total_q + q_begin + qi) * a.Hq + h;
+      const int64_t row = SHARES ? (int64_t)part * n_cols + (c - c0)
+                                 : ((int64_t)part * a.total_q + q_begin + qi) * a.Hq + h;
 #pragma unroll
       for (int w = 0; w < W; ++w) a.part_o[row * D + W * lane + w] = acc[w];
       if (lane == 0) a.part_ml[row] = make_float2(m * kLog2e, l);
@@ -342,9 +345,12 @@ template <> struct PrefillSplit<UKV_DTYPE_F16> {
 //          the tile is a 16-bit pool's, but that FINE stands for the columns' layout alone: P is one fp16 number (11
 //          significant bits beside codes of four to eight), which saves the third of the matrix instructions that
 //          the low parts take, and their registers.
-template <int DT, int D, int WAVES, int CB, bool FINE, bool PARTS, int QF>
+//   SHARES (with PARTS) a piece of the keys, tiles t0 .. t1 - 1: the block's all (np = 1), or some, whose rows, the
+//          block's columns, go to slot `part` of the partials.
+template <int DT, int D, int WAVES, int CB, bool FINE, bool PARTS, int QF, bool SHARES = false>
 __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& a, const int b, const int g,
-                                             const int c0, const int part, const int np, PrefillLds<D>& lds) {
+                                             const int c0, const int part, const int np, PrefillLds<D>& lds,
+                                             const int t0 = 0, const int t1 = 0, const int wave = 0) {
   constexpr bool QUANT = QF != kCache16;
   constexpr bool TWO = FINE && !QUANT;  // weights in two parts
   constexpr int STEPS = D / 32;
@@ -364,9 +370,12 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
   auto& k_s = lds.k_s;
   auto& v_s = lds.v_s;
 
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform
+  int lane = threadIdx.x & 63;
+  // (SHARES: counted anew for each piece, so that nothing that follows from it is held from piece to piece)
+  if constexpr (SHARES)
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  const int wv = SHARES ? wave : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  const int tid = SHARES ? 64 * wv + lane : threadIdx.x;
   const int i16 = lane & 15;
   const int kg = lane >> 4;
 
@@ -386,7 +395,13 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
   int kend = max(0, min(Lk, P0 + min(C, q1)));
   int key_a = 0;  // PARTS: first key of this part; Lk, P0 and kend count from it below
   bool in_parts = false;  // the sequence's keys are in more parts than one (uniform)
-  if constexpr (PARTS) {
+  if constexpr (SHARES) {
+    in_parts = np > 1;
+    key_a = t0 * TK;
+    kend = min(kend, t1 * TK) - key_a;
+    Lk -= key_a;
+    P0 -= key_a;
+  } else if constexpr (PARTS) {
     const int nt = (Lk + TK - 1) / TK;
     if (part >= np) return;  // whole workgroup
     in_parts = np > 1;
@@ -852,10 +867,22 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
     redo_mine = z != 0.f;
   }
   if constexpr (kConvert || FINE || QUANT) {
-    if (__syncthreads_or(redo_mine)) {
-      if (!in_parts) flag_obs_rows<WAVES>(e, b, g, C, max(q0, 0), min(C, q1));  // (none without statistics)
+    bool redo;
+    if constexpr (SHARES) {  // (without the thread's other coordinates, which __syncthreads_or would hold)
+      uint32_t* redo_s = reinterpret_cast<uint32_t*>(&k_s);
+      __syncthreads();  // the last tiles are read
+      const bool any = __any(redo_mine);
+      if (lane == 0) redo_s[wv + lane] = any;
+      __syncthreads();
+      redo = __any(redo_s[lane % WAVES] != 0);
+    } else {
+      redo = __syncthreads_or(redo_mine);
+    }
+    if (redo) {
+      if constexpr (!SHARES)
+        if (!in_parts) flag_obs_rows<WAVES>(e, b, g, C, max(q0, 0), min(C, q1));  // (none without statistics)
       if constexpr (QUANT)
-        prefill_cols_fp32<DT, D, QF>(e, b, g, q_begin, C, P0 + key_a, Lk + key_a, c0, WAVES * CB * 16, wv, WAVES, lane,
+        prefill_cols_fp32<DT, D, QF, SHARES>(e, b, g, q_begin, C, P0 + key_a, Lk + key_a, c0, WAVES * CB * 16, wv, WAVES, lane,
                                      in_parts ? part : -1, key_a, key_a + kend);
       else
         prefill_cols_fp32<DT, D>(e, b, g, q_begin, C, P0 + key_a, Lk + key_a, c0, WAVES * CB * 16, wv, WAVES, lane,
@@ -879,7 +906,8 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
       if (qi >= 0 && qi < C && hh < e.Hq) {
         if (PARTS && in_parts) {
           // (FINE's lift by 2^kLift is in o and l alike: taken off the max)
-          const int64_t row = ((int64_t)part * e.total_q + q_begin + qi) * e.Hq + hh;
+          const int64_t row = SHARES ? (int64_t)part * (WAVES * CB * 16) + (wv * CB + cb) * 16 + col
+                                     : ((int64_t)part * e.total_q + q_begin + qi) * e.Hq + hh;
           float* prow = e.part_o + row * D + i16;
 #pragma unroll
           for (int d = 0; d < NE; ++d) prow[16 * d] = o[cb][d][r];
@@ -890,7 +918,7 @@ __device__ __forceinline__ void prefill_tile(const typename TileArgs<QF>::type& 
         uint16_t* orow = e.out + ((int64_t)(q_begin + qi) * e.Hq + hh) * D + i16;
 #pragma unroll
         for (int d = 0; d < NE; ++d) orow[16 * d] = Elem<DT>::from_float(o[cb][d][r] * inv);
-        if (i16 == 0 && qi >= C - e.obs)  // (never without statistics: obs = 0)
+        if (!SHARES && i16 == 0 && qi >= C - e.obs)  // (never without statistics: obs = 0)
           e.obs_stats[(int64_t)b * e.stats_seq_stride + (int64_t)hh * e.obs + (qi - (C - e.obs))] =
               make_float2(m_col - kLift, lacc[cb][r]);
       }

@@ -1,9 +1,9 @@
 // Chunked prefill attention over the 8-bit paged cache (gfx950): the tiled kernel of paged_prefill.h, whose loader
 // widens codes to the 16-bit values that they are. The tile loop is the 16-bit pool's, so is its bound, the issue of
 // softmax and matrix instructions; the widening adds some thirty VALU instructions a tile of 32 keys to each thread,
-// a tenth of the tile's.
-#include "paged_prefill.h"
+// a tenth of the tile's. Long calls run in shares (quant_shares.hip), cut by the lengths that the device knows.
 #include "quant_rows.h"
+#include "quant_shares.h"
 
 namespace ukv {
 namespace {
@@ -22,6 +22,9 @@ template <int DT> void launch_quant(const QuantPrefillArgs& a, int format, bool 
 
 size_t quant_parts_workspace(int batch, int total_q, int max_chunk, int num_q_heads, int num_kv_heads, int head_dim,
                              int n_rep, int max_blocks) {
+  if (!tiled_shape(head_dim, n_rep)) return 0;
+  Shares s;
+  if (shares_plan(batch, max_chunk, (num_q_heads + n_rep - 1) / n_rep, head_dim, n_rep, max_blocks, s)) return s.total;
   return parts_workspace(batch, total_q, max_chunk, num_q_heads, num_kv_heads, head_dim, n_rep, max_blocks, true);
 }
 
@@ -78,6 +81,10 @@ int quant_prefill(const QuantAttnArgs& x, int total_q, int dtype, int format, vo
   a.max_chunk = x.max_chunk;
   a.scale = x.scale;
   a.scale_log2 = x.scale * kLog2e;
+  Shares shares;
+  if (shares_plan(x.B, x.max_chunk, n_groups, x.D, x.n_rep, x.max_blocks, shares) && workspace &&
+      workspace_bytes >= shares.total && al16(workspace))
+    return launch_shares(a, shares, dtype, format, workspace, stream);
   const bool fine = fine_shape(x.D, x.n_rep);
   const int64_t wgs = plan_launch(a, total_q, true, workspace, workspace_bytes);
   if (wgs > INT32_MAX) return UKV_ERR_INVALID_ARGUMENT;

@@ -677,8 +677,8 @@ int launch(const QuantAttnArgs& x, bool chunk, const WorkspaceLayout& w, int dty
 // workgroups hold 256 columns and more: two queries a sequence on 32/8 heads, 16 sequences of 100-600 tokens 17.8 us
 // against 22.5, 32 of 1-4K 44 against 96, one of 32K 32 against 59. Two need keys enough for the shares, four pages a CU:
 // eight queries 66 against 98 and 41 against 60 us behind the longer ones, but 32 against 24 behind 100-600 tokens and 27
-// against 24 for four of 300-1500. (A second pass over the keys for up to 64 columns paid behind sixteen sequences of
-// 4-32K, 236 us against 348, not behind one of 32K, 66 against 61, or 32 of 1-4K, 120 against 100.)
+// against 24 for four of 300-1500. (A second pass over the keys for up to 64 columns took 236 us behind sixteen sequences of
+// 4-32K, where quant_shares.hip takes 204, 66 against 61 behind one of 32K and 120 against 100 behind 32 of 1-4K.)
 bool chunk_shape(int batch, int max_chunk, int n_rep, int head_dim, int max_blocks) {
   const int64_t columns = (int64_t)max_chunk * n_rep;
   return (head_dim == 64 || head_dim == 128) &&
