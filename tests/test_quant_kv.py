@@ -740,6 +740,8 @@ def test_chunk_longer_than_declared_is_nan_and_written(cuda):
     quant_kv.write_chunk_kv(layer, k, k, table, cu, lens, max_chunk=36)
     rk, _ = quant_kv.read_kv(layer, table, cu, lens, dtype=torch.float16, max_chunk=36, total=70)
     np.testing.assert_array_equal(rk.double().cpu().numpy(), qo.quantise(k.double().cpu().numpy(), "int8")[0])
+    quant_kv.write_chunk_kv(layer, -k, k, table, cu, lens, max_chunk=0)
+    assert torch.equal(quant_kv.read_kv(layer, table, cu, lens, dtype=torch.float16, max_chunk=36, total=70)[0], -rk)
     got = quant_kv.prefill_attention(q, layer, table, cu, lens, softmax_scale=0.1, n_rep=4, max_chunk=36)
     assert torch.isnan(got[:40]).all() and torch.isfinite(got[40:]).all()
     with pytest.raises(RuntimeError, match="max_chunk"):

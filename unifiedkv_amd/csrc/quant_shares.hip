@@ -20,14 +20,17 @@ namespace ukv {
 //
 // 512 queries each behind 6324, 7670, 2480 and 2057 tokens on 28/4 heads 158 us (whole blocks 249), behind 7668 each
 // 242 (261); 16 sequences' 16 drafted tokens behind 4-32K on 32/8 heads 204 us (parts 343), behind 32K each 372 (371);
-// 2048 each behind 0.5-16K 1445 (2035), behind 16K each as long (2090), one alone 540 (590).
+// 2048 each behind 0.5-16K 1445 (2035), behind 16K each 2110 (2115; e4m3 1995 against 1950), one alone 540 (590). A table
+// much wider than its sequences is what this costs most: four 512-token prompts in 2048 pages 46 us (33), unless the host
+// knows the lengths too.
 constexpr int kMaxShareItems = 512;  // (sequence, block) pairs of a launch
 constexpr int kMinShareTiles = 12;   // tiles a share is worth a workgroup for
-// What beginning a block takes, in tiles, ahead of the block's own in the list: with none 178 and 1550 us of the 158 and
-// 1445 above, with 5 164 and 1539.
+// What beginning a block takes, in tiles, ahead of the block's own in the list: with none 178 and 1550 us in place of the
+// 158 and 1445 above, with 5 164 and 1539.
 constexpr int kBlockTiles = 8;
 // Wide tiles of the list, by the table's width, for each workgroup: shorter calls lose more to the pieces' starts and
-// partials than even shares gain (16 x 256 queries behind 1000 tokens 128 us against 114, behind 100-2000 182 against 165).
+// partials than even shares gain (16 x 256 queries behind 1000 tokens 128 us against 114, behind 100-2000 182 against
+// 165).
 constexpr int kMinSlotTiles = 128;
 
 __device__ __forceinline__ int first_lane(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -88,16 +91,16 @@ quant_shares_kernel(const QuantPrefillArgs a) {
     const int u1 = min(all + kBlockTiles, u0 + x1 - x), t0 = max(0, u0 - kBlockTiles), t1 = u1 - kBlockTiles;
     const int C = a.cu_q[b + 1] - a.cu_q[b];
     if (t1 > 0 && C <= a.max_chunk)  // (a longer chunk's rows are the merge's)
-      prefill_tile<DT, D, WAVES, CB, FINE, true, QF, true>(args_again<QuantPrefillArgs>(), b, g, C * a.n_rep - W * (j + 1),
-                                                           2 * w + (x > x0), t0 == 0 && t1 == all ? 1 : 2, lds, t0, t1,
-                                                           wave);
+      prefill_tile<DT, D, WAVES, CB, FINE, true, QF, true>(args_again<QuantPrefillArgs>(), b, g,
+                                                           C * a.n_rep - W * (j + 1), 2 * w + (x > x0),
+                                                           t0 == 0 && t1 == all ? 1 : 2, lds, t0, t1, wave);
     x += u1 - u0;
     __syncthreads();  // the tiles in LDS are read
   }
 }
 
-// A workgroup takes an eighth of the rows of one block (number blockIdx.x / 8, sequence by sequence) in more pieces than
-// one, a group of D / 4 lanes a row: with M the largest of the pieces' m, out = sum(2^(m - M) O) / sum(2^(m - M) l).
+// A workgroup takes an eighth of the rows of one block (number blockIdx.x / 8, sequence by sequence) in more pieces
+// than one, a group of D / 4 lanes a row: with M the largest of the pieces' m, out = sum(2^(m - M) O) / sum(2^(m - M) l).
 template <int DT, int D, int W>
 __global__ void __launch_bounds__(256) quant_shares_merge_kernel(const QuantPrefillArgs a) {
   constexpr int LANES = D / 4, ROWS = 256 / LANES, PER = W / 8;
@@ -158,7 +161,8 @@ __global__ void __launch_bounds__(256) quant_shares_merge_kernel(const QuantPref
 
 namespace {
 
-template <int DT, int D, int CB, bool FINE, int QF> void launch(const QuantPrefillArgs& a, int wgs, hipStream_t stream) {
+template <int DT, int D, int CB, bool FINE, int QF>
+void launch(const QuantPrefillArgs& a, int wgs, hipStream_t stream) {
   constexpr int WV = UKV_PREFILL_WAVES;
   hipLaunchKernelGGL((quant_shares_kernel<DT, D, WV, CB, FINE, QF>), dim3(wgs), dim3(64 * WV), 0, stream, a);
   hipLaunchKernelGGL((quant_shares_merge_kernel<DT, D, WV * CB * 16>), dim3(8 * a.B * a.share_blocks * a.n_groups),
@@ -193,8 +197,8 @@ bool shares_plan(int batch, int max_chunk, int n_groups, int head_dim, int n_rep
     return false;
   const double list = (double)(batch * n_groups * blocks) * (double)(tiles + kBlockTiles) *
                       (s.column_blocks == wide ? 1.0 : narrow);
-  // (With no more keys than twice the chunk's the blocks differ by a factor of two and more, and the host's plan runs the
-  // longest first: 4 x 4096 tokens without a prefix 553 us, 627 in shares.)
+  // (With no more keys than twice the chunk's the blocks differ by a factor of two and more, and the host's plan runs
+  // the longest first: 4 x 4096 tokens without a prefix 553 us, 627 in shares.)
   if (list < kMinSlotTiles * s.wgs || (int64_t)max_blocks * 16 <= 2 * (int64_t)max_chunk) return false;
   s.blocks = (int)blocks;
   const size_t rows = 2 * (size_t)s.wgs * UKV_PREFILL_WAVES * s.column_blocks * 16;

@@ -148,6 +148,8 @@ def write_chunk_kv(layer: QuantLayer, k_new: torch.Tensor, v_new: torch.Tensor, 
     cu, lens, bt = _i32(cu_seqlens_q, dev), _i32(kv_lens, dev), _i32(block_table, dev)
     B = _batch(cu, lens, bt)
     mc = _max_chunk(cu_seqlens_q, max_chunk, chunk_lens)
+    if chunk_lens is None:
+        mc = max(mc, 1)  # (sizes the launch alone: rows beyond it are written too)
     _write(layer, k_new, v_new, bt, cu, lens, 0, B, mc)
 
 
