@@ -62,7 +62,7 @@ struct QuantPrefillArgs : PrefillArgs {
   const uint8_t* vs;
   int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
   int share_blocks;    // shares (quant_prefill.hip): query blocks of a pair at most
-  int32_t* share_map;  // [B * share_blocks + 2]
+  int32_t* share_map;  // [B * share_blocks + 1] starts, the shares G, [G] the blocks cut behind them
 };
 template <int QF> struct TileArgs { typedef QuantPrefillArgs type; };
 template <> struct TileArgs<kCache16> { typedef PrefillArgs type; };

@@ -82,6 +82,7 @@ quant_shares_kernel(const QuantPrefillArgs a) {
   if ((int)blockIdx.x >= G) return;
   const int w = (int)(blockIdx.x & 7) * (G >> 3) + (int)(blockIdx.x >> 3);  // an XCD's shares next to each other
   const int x0 = first_lane(share_start(w, T, G)), x1 = first_lane(share_start(w + 1, T, G));
+  int cut = -1;  // the block that the share holds the first of several pieces of (one at most, its last)
   for (int x = x0; x < x1;) {
     const int b = last_at(starts, a.n_groups, x, 0, a.B, nb);
     const int s_b = first_lane(starts[b * nb]), u_b = first_lane(starts[(b + 1) * nb]) - s_b;
@@ -94,33 +95,42 @@ quant_shares_kernel(const QuantPrefillArgs a) {
       prefill_tile<DT, D, WAVES, CB, FINE, true, QF, true>(args_again<QuantPrefillArgs>(), b, g,
                                                            C * a.n_rep - W * (j + 1), 2 * w + (x > x0),
                                                            t0 == 0 && t1 == all ? 1 : 2, lds, t0, t1, wave);
+    if (t1 > 0 && t0 == 0 && t1 < all) cut = i * a.n_groups + g;
     x += u1 - u0;
     __syncthreads();  // the tiles in LDS are read
   }
+  int lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  const QuantPrefillArgs& e = args_again<QuantPrefillArgs>();
+  if (wave == 0 && lane == 0) e.share_map[e.B * e.share_blocks + 2 + w] = cut;
 }
 
-// A workgroup takes an eighth of the rows of one block (number blockIdx.x / 8, sequence by sequence) in more pieces
-// than one, a group of D / 4 lanes a row: with M the largest of the pieces' m, out = sum(2^(m - M) O) / sum(2^(m - M) l).
+// Workgroup w * SUB + s takes part s of the rows of the block that share w holds the first piece of, a group of D / 4
+// lanes a row: with M the largest of the pieces' m, out = sum(2^(m - M) O) / sum(2^(m - M) l). Bound: HBM, where the
+// partials go. The last workgroups write the chunks longer than declared.
+template <int D, int W> constexpr int kMergeSub = W / (2 * (256 / (D / 4)));
 template <int DT, int D, int W>
-__global__ void __launch_bounds__(256) quant_shares_merge_kernel(const QuantPrefillArgs a) {
-  constexpr int LANES = D / 4, ROWS = 256 / LANES, PER = W / 8;
-  const int item = blockIdx.x >> 3, sub = blockIdx.x & 7, nb = a.share_blocks, n = a.B * nb;
-  const int i = item / a.n_groups, g = item - i * a.n_groups, b = i / nb, j = i - b * nb;
-  const int32_t* starts = a.share_map;
-  const int all = starts[i + 1] - starts[i] - kBlockTiles, T = a.n_groups * starts[n], G = starts[n + 1];
-  if (all < 0) return;
-  const int s_b = starts[b * nb], u_b = starts[(b + 1) * nb] - s_b;
-  const int begin = a.n_groups * s_b + g * u_b + starts[i] - s_b, X = begin + kBlockTiles;  // the block, its first tile
-  const int w0 = share_of(X, T, G), w1 = share_of(X + all - 1, T, G);
-  const int q_begin = a.cu_q[b], C = a.cu_q[b + 1] - q_begin, Lk = kv_len_of(a, b);
-  if (C > a.max_chunk) {  // longer than declared: NaN, an eighth of the rows each
-    if (j == 0) prefill_nan_rows<4>(a, b, g, (int)((int64_t)C * sub / 8), (int)((int64_t)C * (sub + 1) / 8));
+__global__ void __launch_bounds__(256) quant_shares_merge_kernel(const QuantPrefillArgs a, const int wgs) {
+  constexpr int LANES = D / 4, ROWS = 256 / LANES, SUB = kMergeSub<D, W>, PER = W / SUB;
+  const int w0 = blockIdx.x / SUB, sub = blockIdx.x % SUB, nb = a.share_blocks, n = a.B * nb;
+  if (w0 >= wgs) {
+    const int pair = blockIdx.x - wgs * SUB, b = pair / a.n_groups, C = a.cu_q[b + 1] - a.cu_q[b];
+    if (C > a.max_chunk) prefill_nan_rows<4>(a, b, pair % a.n_groups, 0, C);
     return;
   }
-  if (w0 == w1) return;  // written whole
+  const int32_t* starts = a.share_map;
+  const int item = starts[n + 2 + w0], T = a.n_groups * starts[n], G = starts[n + 1];
+  if (w0 >= G || item < 0) return;
+  const int i = item / a.n_groups, g = item - i * a.n_groups, b = i / nb, j = i - b * nb;
+  const int all = starts[i + 1] - starts[i] - kBlockTiles;
+  const int s_b = starts[b * nb], u_b = starts[(b + 1) * nb] - s_b;
+  const int begin = a.n_groups * s_b + g * u_b + starts[i] - s_b, X = begin + kBlockTiles;  // the block, its first tile
+  const int q_begin = a.cu_q[b], C = a.cu_q[b + 1] - q_begin, Lk = kv_len_of(a, b);
   const int c0 = C * a.n_rep - W * (j + 1), dq = threadIdx.x % LANES;
   const int slot0 = 2 * w0 + (begin > share_start(w0, T, G));
-  for (int col = sub * PER + threadIdx.x / LANES; col < (sub + 1) * PER; col += ROWS) {
+#pragma unroll
+  for (int k = 0; k < PER / ROWS; ++k) {
+    const int col = sub * PER + k * ROWS + threadIdx.x / LANES;
     const int c = c0 + col, qi = c / a.n_rep, h = g * a.n_rep + c - qi * a.n_rep;
     if (c < 0 || h >= a.Hq) continue;
     const int pos = Lk - C + qi;
@@ -128,24 +138,24 @@ __global__ void __launch_bounds__(256) quant_shares_merge_kernel(const QuantPref
     const int n_pieces = pos < 0 ? 0 : share_of(min(X + pos / kTileKeys, X + all - 1), T, G) - w0 + 1;
     float M = kNegFltMax, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < n_pieces; p0 += 4) {
-      float2 ml[4];
-      f32x4 o[4];
+    for (int p0 = 0; p0 < n_pieces; p0 += 2) {  // (two in most blocks)
+      float2 ml[2];
+      f32x4 o[2];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         const int p = min(p0 + u, n_pieces - 1);
         const int64_t at = (int64_t)(p == 0 ? slot0 : 2 * (w0 + p)) * W + col;
         ml[u] = a.part_ml[at];
         o[u] = *reinterpret_cast<const f32x4*>(a.part_o + at * D + 4 * dq);
         if (p0 + u >= n_pieces) ml[u] = make_float2(kNegFltMax, 0.f);
       }
-      const float top = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+      const float top = fmaxf(M, fmaxf(ml[0].x, ml[1].x));
       const float f = fast_exp2(M - top);
       l *= f;
       acc *= f;
       M = top;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         if (p0 + u >= n_pieces) continue;
         const float wt = fast_exp2(ml[u].x - M);
         l += wt * ml[u].y;
@@ -165,8 +175,9 @@ template <int DT, int D, int CB, bool FINE, int QF>
 void launch(const QuantPrefillArgs& a, int wgs, hipStream_t stream) {
   constexpr int WV = UKV_PREFILL_WAVES;
   hipLaunchKernelGGL((quant_shares_kernel<DT, D, WV, CB, FINE, QF>), dim3(wgs), dim3(64 * WV), 0, stream, a);
-  hipLaunchKernelGGL((quant_shares_merge_kernel<DT, D, WV * CB * 16>), dim3(8 * a.B * a.share_blocks * a.n_groups),
-                     dim3(256), 0, stream, a);
+  constexpr int W = WV * CB * 16;
+  hipLaunchKernelGGL((quant_shares_merge_kernel<DT, D, W>), dim3(wgs * kMergeSub<D, W> + a.B * a.n_groups), dim3(256), 0,
+                     stream, a, wgs);
 }
 template <int DT, int D, bool FINE, int QF>
 void launch_blocks(const QuantPrefillArgs& a, const Shares& s, hipStream_t stream) {
@@ -204,7 +215,7 @@ bool shares_plan(int batch, int max_chunk, int n_groups, int head_dim, int n_rep
   const size_t rows = 2 * (size_t)s.wgs * UKV_PREFILL_WAVES * s.column_blocks * 16;
   s.ml_off = up256(rows * head_dim * sizeof(float));
   s.map_off = s.ml_off + up256(rows * sizeof(float2));
-  s.total = s.map_off + up256((batch * blocks + 2) * sizeof(int32_t));
+  s.total = s.map_off + up256((batch * blocks + 2 + s.wgs) * sizeof(int32_t));
   return true;
 }
 
