@@ -15,8 +15,8 @@ namespace ukv {
 // piece is written as by a launch without shares; the pieces of the others leave their partials (m, l, O) in two slots
 // of each workgroup, and quant_shares_merge_kernel adds them up. A share's first and last pieces alone can be parts of
 // blocks: slot 2 w for a piece that begins the share, 2 w + 1 for one that does not. Bound, like the tiled kernel, by
-// the issue of softmax and matrix instructions, then by the partials (two of 100 KB a workgroup at 128 dims) and their
-// merge, 4-10 us.
+// the issue of softmax and matrix instructions, then by the partials, up to two of 200 KB a workgroup at 128 dims, and
+// their merge, 15-20 us at 5 TB/s where 400 of them are full.
 //
 // 512 queries each behind 6324, 7670, 2480 and 2057 tokens on 28/4 heads 158 us (whole blocks 249), behind 7668 each
 // 242 (261); 16 sequences' 16 drafted tokens behind 4-32K on 32/8 heads 204 us (parts 343), behind 32K each 372 (371);
