@@ -62,8 +62,8 @@ def log(*a):
 
 # The sources the decode kernels are compiled from: a PMC summary applies to a build only when
 # these hash the same as when it was measured.
-DECODE_SOURCES = ("unifiedkv_amd/csrc/page16_decode.hip", "unifiedkv_amd/csrc/ukv_common.h", "include/ukv.h",
-                  "unifiedkv_amd/_build.py")
+DECODE_SOURCES = ("unifiedkv_amd/csrc/page16_decode.hip", "unifiedkv_amd/csrc/page16_split.h",
+                  "unifiedkv_amd/csrc/ukv_common.h", "include/ukv.h", "unifiedkv_amd/_build.py")
 
 
 def decode_sources_sha256() -> str:
